@@ -55,7 +55,13 @@ typedef enum {
   B200ATTN_ERR_DEVICE = -12      /* current device is not compute capability 10.x */
 } b200attn_status;
 
-typedef enum { B200ATTN_F16 = 0, B200ATTN_BF16 = 1, B200ATTN_F32 = 2 /* RMSNorm only */ } b200attn_dtype;
+typedef enum {
+  B200ATTN_F16 = 0,
+  B200ATTN_BF16 = 1,
+  B200ATTN_F32 = 2,     /* RMSNorm only */
+  B200ATTN_E4M3 = 3,    /* 8-bit caches only */
+  B200ATTN_I8 = 4       /* 8-bit caches only */
+} b200attn_dtype;
 
 typedef enum {
   B200ATTN_DENSE = 0,       /* every (causally) visible key */
@@ -395,6 +401,175 @@ typedef struct {
  * reference, whose tests rebuild the whole cache instead
  * (flash_attn_triton/flash_attn_decoding_sparse.py:445-466). */
 int b200attn_kv_append(const b200attn_kv_append_args* args, b200attn_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Paged KV cache held in 8 bits.
+ *
+ * k_pages / v_pages are pools [num_pages, page_size, heads_kv, head_dim] of
+ * E4M3 or I8 numbers (any strides that are multiples of 16, so a pool whose
+ * heads lie outside its tokens does as well), k_scales / v_scales fp32 pools
+ * [num_pages, page_size / block_tokens, heads_kv]: element (page, t, h, d) stands
+ * for number * scale[page][t / block_tokens][h].  block_tokens is 16, 32, 64 or
+ * 128 and divides page_size.  page_table [batch, max_pages_per_seq] lists the
+ * pages of each sequence; an entry outside [0, num_pages) names no page: its keys
+ * are not attended to and rows that would go there are not stored.
+ * The reference keeps its caches in 16 bits and padded (flash_attn_decoding.py:62-69).
+ * ---------------------------------------------------------------------- */
+typedef struct {
+  const void* q;               /* [batch, queries, heads_q, head_dim] */
+  const void* k_pages;
+  const void* v_pages;
+  const float* k_scales;
+  const float* v_scales;
+  void* o;                     /* like q */
+  int32_t dtype;               /* of q and o: F16 or BF16 */
+  int32_t cache_dtype;         /* E4M3 or I8 */
+  int32_t batch, queries;      /* queries: the newest tokens of each sequence, >= 1 */
+  int32_t heads_q, heads_kv, head_dim;
+  int32_t page_size;           /* a multiple of 16 */
+  int32_t block_tokens;
+  int32_t num_pages, max_pages_per_seq;
+  int32_t max_seqlen;          /* upper bound on the lengths; longer ones are cut there */
+  const int32_t* page_table;   /* int32 [batch, max_pages_per_seq] */
+  const int32_t* seqlens;      /* int32 [batch]: keys of each sequence, the queries' own included */
+  int64_t q_stride_b, q_stride_t, q_stride_h;
+  int64_t k_stride_page, k_stride_t, k_stride_h;
+  int64_t v_stride_page, v_stride_t, v_stride_h;
+  int64_t ks_stride_page, ks_stride_blk, ks_stride_h;
+  int64_t vs_stride_page, vs_stride_blk, vs_stride_h;
+  int64_t o_stride_b, o_stride_t, o_stride_h;
+  float softmax_scale;         /* natural scale */
+  int32_t chunk_tokens;        /* keys per split, a multiple of 128; 0: chosen from the sizes */
+  void* workspace;
+  size_t workspace_bytes;
+  int32_t* status_word;        /* nullable; as in b200attn_decode_args */
+} b200attn_paged_decode_8bit_args;
+
+size_t b200attn_paged_decode_8bit_workspace_bytes(const b200attn_paged_decode_8bit_args* args);
+
+/* Split-KV GQA attention of the newest tokens over an 8-bit paged cache: query i
+ * of `queries` attends to keys t < len - queries + 1 + i (the token itself and
+ * what came before it), len cut at max_seqlen and at the row of the page table.
+ * A query without a visible key gives 0.  Scores, softmax statistics and sums
+ * are fp32; Q enters the products as fp16 (bf16 rows scaled by a power of two
+ * first), the cached numbers as fp16, which holds them exactly. */
+int b200attn_paged_decode_8bit_fwd(const b200attn_paged_decode_8bit_args* args, b200attn_stream_t stream);
+
+typedef struct {
+  const void* new_k;           /* [tokens, heads, head_dim] F16 or BF16 rows */
+  const void* new_v;
+  void* k_pages;
+  void* v_pages;
+  float* k_scales;
+  float* v_scales;
+  int32_t dtype, cache_dtype;
+  int32_t batch, heads, head_dim;
+  int64_t tokens;              /* rows of new_k / new_v */
+  int32_t page_size, block_tokens;
+  int32_t num_pages, max_pages_per_seq;
+  const int32_t* page_table;   /* int32 [batch, max_pages_per_seq] */
+  const int32_t* seqlens;      /* int32 [batch]: tokens each sequence holds before the call */
+  const int32_t* cu_new;       /* int32 [batch+1]: the new rows of each sequence; NULL: one each */
+  int64_t nk_stride_t, nk_stride_h;
+  int64_t nv_stride_t, nv_stride_h;
+  int64_t k_stride_page, k_stride_t, k_stride_h;
+  int64_t v_stride_page, v_stride_t, v_stride_h;
+  int64_t ks_stride_page, ks_stride_blk, ks_stride_h;
+  int64_t vs_stride_page, vs_stride_blk, vs_stride_h;
+} b200attn_kv_append_8bit_args;
+
+/* New K / V rows quantised into the cache at positions len_b, len_b + 1, ... of each
+ * sequence (rows past the end of the page table's row are not stored, nor are those
+ * of a negative length).  A block's scale is the smallest power of two with which its
+ * largest element fits (448 for E4M3, 127 for I8), 0 for a block of zeros, NaN if an
+ * element is not finite; rows that join a block already begun raise its scale where
+ * they have to, and the rows it holds are then rounded to the new one.  Powers of two
+ * divide exactly, so E4M3 rows lose nothing in that step unless they fall into the
+ * type's subnormals.  A page that is written must belong to one row of the table only. */
+int b200attn_kv_append_8bit(const b200attn_kv_append_8bit_args* args, b200attn_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Pages of a cache: hand-out, forking, freeing, compaction, on the device.
+ *
+ * page_table int32 [slots, max_pages_per_seq]: the pages of each slot's sequence,
+ * -1 (or any number outside [0, num_pages)) where there is none; page_refs int32
+ * [num_pages]: how many rows hold a page, <= 0 for a free one (a caller may add to
+ * the count of a page it wants kept).  The results are new tensors, which must not
+ * overlap the ones read; entries without a page are -1 there.  Pages are handed out
+ * lowest number first, so results are a pure function of the inputs.  The reference
+ * has no counterpart: its caches are padded and never shared.
+ * ---------------------------------------------------------------------- */
+typedef struct {               /* one tensor [num_pages, ...] whose pages are blocks of memory */
+  void* base;
+  int64_t page_bytes;          /* bytes of a page, a multiple of 4; base is 4-byte aligned */
+  int64_t stride_bytes;        /* from one page to the next, a multiple of 4 and >= page_bytes */
+} b200attn_page_pool;
+
+typedef struct {
+  const int32_t* page_table;
+  const int32_t* seqlens;      /* int32 [slots]: tokens each slot holds */
+  const int32_t* page_refs;
+  const int32_t* new_tokens;   /* int32 [slots]: tokens to come */
+  int32_t* page_table_out;
+  int32_t* page_refs_out;
+  int32_t* missing_out;        /* int32 [1]: pages that could not be given */
+  int32_t slots, max_pages_per_seq, num_pages, page_size;
+  void* workspace;
+  size_t workspace_bytes;
+} b200attn_pages_grow_args;
+
+size_t b200attn_pages_grow_workspace_bytes(const b200attn_pages_grow_args* args);
+
+/* Pages for the tokens to come: entries i < ceil((seqlens + new_tokens) / page_size)
+ * of a row that hold no page get one, in the order of slots and entries, until none
+ * is free. */
+int b200attn_pages_grow(const b200attn_pages_grow_args* args, b200attn_stream_t stream);
+
+typedef struct {
+  const int32_t* page_table;
+  const int32_t* seqlens;
+  const int32_t* page_refs;
+  const int32_t* parents;      /* int32 [slots] */
+  int32_t* page_table_out;
+  int32_t* seqlens_out;
+  int32_t* page_refs_out;
+  int32_t* missing_out;        /* int32 [1]: copies that found no free page */
+  const b200attn_page_pool* pools;  /* HOST array of n_pools entries, read during the call */
+  int32_t n_pools;
+  int32_t slots, max_pages_per_seq, num_pages, page_size;
+  void* workspace;
+  size_t workspace_bytes;
+} b200attn_pages_fork_args;
+
+size_t b200attn_pages_fork_workspace_bytes(const b200attn_pages_fork_args* args);
+
+/* Every slot b becomes the sequence that slot parents[b] held (a beam search step, a
+ * fork, a reordering), all at once; a parent outside [0, slots) frees the slot.  One
+ * slot keeps each surviving row whole (its own slot if that stays, else the lowest one
+ * that takes it); the others share its full pages and get a copy, in every pool, of the
+ * last page if that is only partly filled.  Pages that no row holds any more are free,
+ * also for the copies of this call.  A copy that finds no free page is left out: its
+ * entry is -1, its length is cut to the full pages and missing_out counts it. */
+int b200attn_pages_fork(const b200attn_pages_fork_args* args, b200attn_stream_t stream);
+
+typedef struct {
+  const int32_t* page_table;
+  const int32_t* page_refs;
+  int32_t* page_table_out;
+  int32_t* page_refs_out;
+  int32_t* live_out;           /* int32 [1]: pages in use */
+  const b200attn_page_pool* pools;  /* HOST array, as above */
+  int32_t n_pools;
+  int32_t slots, max_pages_per_seq, num_pages;
+  void* workspace;
+  size_t workspace_bytes;
+} b200attn_pages_compact_args;
+
+size_t b200attn_pages_compact_workspace_bytes(const b200attn_pages_compact_args* args);
+
+/* The pages in use moved to the front of every pool: with n of them, those at n and
+ * beyond take, in order, the free places below n. */
+int b200attn_pages_compact(const b200attn_pages_compact_args* args, b200attn_stream_t stream);
 
 /* ------------------------------------------------------------------------
  * RMSNorm over the last dimension of a [rows, dim] view (the op in front of the

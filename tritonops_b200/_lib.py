@@ -10,7 +10,7 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "csrc", "libb200attn.so")
 
-F16, BF16, F32 = 0, 1, 2
+F16, BF16, F32, E4M3, I8 = 0, 1, 2, 3, 4
 DENSE, WINDOW, BLOCK_LIST = 0, 1, 2
 
 i32, i64, f32, vp = C.c_int32, C.c_int64, C.c_float, C.c_void_p
@@ -92,6 +92,60 @@ class PagedDecodeArgs(C.Structure):
     ]
 
 
+class PagedDecode8bitArgs(C.Structure):
+    _fields_ = [
+        ("q", vp), ("k_pages", vp), ("v_pages", vp), ("k_scales", vp), ("v_scales", vp), ("o", vp),
+        ("dtype", i32), ("cache_dtype", i32), ("batch", i32), ("queries", i32),
+        ("heads_q", i32), ("heads_kv", i32), ("head_dim", i32),
+        ("page_size", i32), ("block_tokens", i32), ("num_pages", i32), ("max_pages_per_seq", i32),
+        ("max_seqlen", i32), ("page_table", vp), ("seqlens", vp),
+        ("q_stride_b", i64), ("q_stride_t", i64), ("q_stride_h", i64),
+    ] + [(f"{n}_stride_{a}", i64) for n in ("k", "v") for a in ("page", "t", "h")] + [
+        (f"{n}_stride_{a}", i64) for n in ("ks", "vs") for a in ("page", "blk", "h")] + [
+        ("o_stride_b", i64), ("o_stride_t", i64), ("o_stride_h", i64),
+        ("softmax_scale", f32), ("chunk_tokens", i32),
+        ("workspace", vp), ("workspace_bytes", C.c_size_t), ("status_word", vp),
+    ]
+
+
+class KvAppend8bitArgs(C.Structure):
+    _fields_ = [
+        ("new_k", vp), ("new_v", vp), ("k_pages", vp), ("v_pages", vp), ("k_scales", vp), ("v_scales", vp),
+        ("dtype", i32), ("cache_dtype", i32), ("batch", i32), ("heads", i32), ("head_dim", i32), ("tokens", i64),
+        ("page_size", i32), ("block_tokens", i32), ("num_pages", i32), ("max_pages_per_seq", i32),
+        ("page_table", vp), ("seqlens", vp), ("cu_new", vp),
+        ("nk_stride_t", i64), ("nk_stride_h", i64), ("nv_stride_t", i64), ("nv_stride_h", i64),
+    ] + [(f"{n}_stride_{a}", i64) for n in ("k", "v") for a in ("page", "t", "h")] + [
+        (f"{n}_stride_{a}", i64) for n in ("ks", "vs") for a in ("page", "blk", "h")]
+
+
+class PagePool(C.Structure):
+    _fields_ = [("base", vp), ("page_bytes", i64), ("stride_bytes", i64)]
+
+
+class PagesGrowArgs(C.Structure):
+    _fields_ = [("page_table", vp), ("seqlens", vp), ("page_refs", vp), ("new_tokens", vp),
+                ("page_table_out", vp), ("page_refs_out", vp), ("missing_out", vp),
+                ("slots", i32), ("max_pages_per_seq", i32), ("num_pages", i32), ("page_size", i32),
+                ("workspace", vp), ("workspace_bytes", C.c_size_t)]
+
+
+class PagesForkArgs(C.Structure):
+    _fields_ = [("page_table", vp), ("seqlens", vp), ("page_refs", vp), ("parents", vp),
+                ("page_table_out", vp), ("seqlens_out", vp), ("page_refs_out", vp), ("missing_out", vp),
+                ("pools", C.POINTER(PagePool)), ("n_pools", i32),
+                ("slots", i32), ("max_pages_per_seq", i32), ("num_pages", i32), ("page_size", i32),
+                ("workspace", vp), ("workspace_bytes", C.c_size_t)]
+
+
+class PagesCompactArgs(C.Structure):
+    _fields_ = [("page_table", vp), ("page_refs", vp),
+                ("page_table_out", vp), ("page_refs_out", vp), ("live_out", vp),
+                ("pools", C.POINTER(PagePool)), ("n_pools", i32),
+                ("slots", i32), ("max_pages_per_seq", i32), ("num_pages", i32),
+                ("workspace", vp), ("workspace_bytes", C.c_size_t)]
+
+
 class WindowBlocksPrefillArgs(C.Structure):
     _fields_ = [("block_idx", vp), ("block_cnt", vp),
                 ("batch", i32), ("heads", i32), ("n_qblocks", i32), ("max_nnz", i32),
@@ -143,6 +197,15 @@ SYMBOLS = {
     "b200attn_kv_append": (C.c_int, [C.POINTER(KvAppendArgs), vp]),
     "b200attn_paged_decode_workspace_bytes": (C.c_size_t, [C.POINTER(PagedDecodeArgs)]),
     "b200attn_paged_decode_fwd": (C.c_int, [C.POINTER(PagedDecodeArgs), vp]),
+    "b200attn_paged_decode_8bit_workspace_bytes": (C.c_size_t, [C.POINTER(PagedDecode8bitArgs)]),
+    "b200attn_paged_decode_8bit_fwd": (C.c_int, [C.POINTER(PagedDecode8bitArgs), vp]),
+    "b200attn_kv_append_8bit": (C.c_int, [C.POINTER(KvAppend8bitArgs), vp]),
+    "b200attn_pages_grow_workspace_bytes": (C.c_size_t, [C.POINTER(PagesGrowArgs)]),
+    "b200attn_pages_grow": (C.c_int, [C.POINTER(PagesGrowArgs), vp]),
+    "b200attn_pages_fork_workspace_bytes": (C.c_size_t, [C.POINTER(PagesForkArgs)]),
+    "b200attn_pages_fork": (C.c_int, [C.POINTER(PagesForkArgs), vp]),
+    "b200attn_pages_compact_workspace_bytes": (C.c_size_t, [C.POINTER(PagesCompactArgs)]),
+    "b200attn_pages_compact": (C.c_int, [C.POINTER(PagesCompactArgs), vp]),
     "b200attn_window_blocks_prefill_max_nnz": (i32, [i32, i32, i32, i32]),
     "b200attn_window_blocks_prefill": (C.c_int, [C.POINTER(WindowBlocksPrefillArgs), vp]),
     "b200attn_window_blocks_decode": (C.c_int, [C.POINTER(WindowBlocksDecodeArgs), vp]),

@@ -130,6 +130,47 @@ int b200attn_topk_blocks(const b200attn_topk_blocks_args* args, b200attn_stream_
   return topk_blocks(args, (cudaStream_t)stream);
 }
 
+size_t b200attn_paged_decode_8bit_workspace_bytes(const b200attn_paged_decode_8bit_args* args) {
+  return paged_decode_8bit_workspace_bytes(args);
+}
+
+int b200attn_paged_decode_8bit_fwd(const b200attn_paged_decode_8bit_args* args, b200attn_stream_t stream) {
+  set_launch_count(0);
+  return paged_decode_8bit_fwd(args, (cudaStream_t)stream);
+}
+
+int b200attn_kv_append_8bit(const b200attn_kv_append_8bit_args* args, b200attn_stream_t stream) {
+  set_launch_count(0);
+  return kv_append_8bit(args, (cudaStream_t)stream);
+}
+
+size_t b200attn_pages_grow_workspace_bytes(const b200attn_pages_grow_args* args) {
+  return pages_grow_workspace_bytes(args);
+}
+
+int b200attn_pages_grow(const b200attn_pages_grow_args* args, b200attn_stream_t stream) {
+  set_launch_count(0);
+  return pages_grow(args, (cudaStream_t)stream);
+}
+
+size_t b200attn_pages_fork_workspace_bytes(const b200attn_pages_fork_args* args) {
+  return pages_fork_workspace_bytes(args);
+}
+
+int b200attn_pages_fork(const b200attn_pages_fork_args* args, b200attn_stream_t stream) {
+  set_launch_count(0);
+  return pages_fork(args, (cudaStream_t)stream);
+}
+
+size_t b200attn_pages_compact_workspace_bytes(const b200attn_pages_compact_args* args) {
+  return pages_compact_workspace_bytes(args);
+}
+
+int b200attn_pages_compact(const b200attn_pages_compact_args* args, b200attn_stream_t stream) {
+  set_launch_count(0);
+  return pages_compact(args, (cudaStream_t)stream);
+}
+
 int b200attn_rmsnorm_fwd(const b200attn_rmsnorm_fwd_args* args, b200attn_stream_t stream) {
   set_launch_count(0);
   return rmsnorm_fwd(args, (cudaStream_t)stream);

@@ -41,6 +41,15 @@ int window_blocks_prefill(const b200attn_window_blocks_prefill_args* a, cudaStre
 int window_blocks_decode(const b200attn_window_blocks_decode_args* a, cudaStream_t stream);
 int topk_blocks(const b200attn_topk_blocks_args* a, cudaStream_t stream);
 int selftest_bounded_wait(int32_t* status_word, long long budget_cycles, long long* waited_cycles, cudaStream_t stream);
+size_t paged_decode_8bit_workspace_bytes(const b200attn_paged_decode_8bit_args* a);
+int paged_decode_8bit_fwd(const b200attn_paged_decode_8bit_args* a, cudaStream_t stream);
+int kv_append_8bit(const b200attn_kv_append_8bit_args* a, cudaStream_t stream);
+size_t pages_grow_workspace_bytes(const b200attn_pages_grow_args* a);
+int pages_grow(const b200attn_pages_grow_args* a, cudaStream_t stream);
+size_t pages_fork_workspace_bytes(const b200attn_pages_fork_args* a);
+int pages_fork(const b200attn_pages_fork_args* a, cudaStream_t stream);
+size_t pages_compact_workspace_bytes(const b200attn_pages_compact_args* a);
+int pages_compact(const b200attn_pages_compact_args* a, cudaStream_t stream);
 int rmsnorm_fwd(const b200attn_rmsnorm_fwd_args* a, cudaStream_t stream);
 size_t rmsnorm_bwd_workspace_bytes(const b200attn_rmsnorm_bwd_args* a);
 int rmsnorm_bwd(const b200attn_rmsnorm_bwd_args* a, cudaStream_t stream);

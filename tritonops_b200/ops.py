@@ -13,8 +13,8 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from ._lib import (BLOCK_LIST, DENSE, WINDOW, DecodeArgs, KvAppendArgs, KvPackArgs, PagedDecodeArgs,
-                   PrefillArgs, PrefillBwdArgs, RmsNormBwdArgs, RmsNormFwdArgs, TopkBlocksArgs,
+from ._lib import (BLOCK_LIST, DENSE, WINDOW, DecodeArgs, KvAppend8bitArgs, KvAppendArgs, KvPackArgs, PagedDecode8bitArgs,
+                   PagedDecodeArgs, PagePool, PagesCompactArgs, PagesForkArgs, PagesGrowArgs, PrefillArgs, PrefillBwdArgs, RmsNormBwdArgs, RmsNormFwdArgs, TopkBlocksArgs,
                    WindowBlocksDecodeArgs, WindowBlocksPrefillArgs)
 
 LOG2E = 1.4426950408889634
@@ -577,6 +577,213 @@ def append_kv(k_cache: Tensor, v_cache: Tensor, new_k: Tensor, new_v: Tensor, se
     with torch.cuda.device(k_cache.device):
         _lib.check(_lib.lib().b200attn_kv_append(C.byref(a), _stream(k_cache)))
     _count()
+
+
+# --------------------------------------------------------------------------
+# paged cache in 8 bits
+# --------------------------------------------------------------------------
+_DT_8BIT = {torch.float8_e4m3fn: _lib.E4M3, torch.int8: _lib.I8}
+
+
+def _check_8bit_cache(k_pages, v_pages, k_scales, v_scales, page_table, *others):
+    """(cache dtype code, tokens of a scale block) of the pools and scales of a cache."""
+    _need_cuda(k_pages, v_pages, k_scales, v_scales, page_table, *others)
+    for t in (k_pages, v_pages, k_scales, v_scales, page_table, *others):
+        if t is not None and t.device != k_pages.device:
+            raise ValueError("b200attn: the cache and its operands must be on one device")
+    if k_pages.dtype not in _DT_8BIT or v_pages.dtype != k_pages.dtype:
+        raise ValueError("b200attn: an 8-bit cache holds float8_e4m3fn or int8 pools, K and V alike")
+    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
+        raise ValueError("b200attn: pools are [num_pages, page_size, Hkv, D], K and V alike")
+    if k_pages.stride(3) != 1 or v_pages.stride(3) != 1:
+        raise ValueError("b200attn: the rows of a pool must be contiguous")
+    if k_scales.dtype != torch.float32 or v_scales.dtype != torch.float32:
+        raise ValueError("b200attn: scales are float32")
+    pages, size, heads, _ = k_pages.shape
+    if k_scales.dim() != 3 or v_scales.shape != k_scales.shape or k_scales.shape[0] != pages \
+            or k_scales.shape[2] != heads or k_scales.shape[1] == 0 or size % k_scales.shape[1] != 0:
+        raise ValueError("b200attn: scales are [num_pages, page_size // block, Hkv], K and V alike")
+    if page_table.dim() != 2:
+        raise ValueError("b200attn: page_table is [batch, max_pages]")
+    return _DT_8BIT[k_pages.dtype], size // k_scales.shape[1]
+
+
+def _pool_strides(a, k, v, ks, vs):
+    a.k_stride_page, a.k_stride_t, a.k_stride_h = k.stride()[:3]
+    a.v_stride_page, a.v_stride_t, a.v_stride_h = v.stride()[:3]
+    a.ks_stride_page, a.ks_stride_blk, a.ks_stride_h = ks.stride()
+    a.vs_stride_page, a.vs_stride_blk, a.vs_stride_h = vs.stride()
+
+
+def paged_decode_8bit(q: Tensor, k_pages: Tensor, v_pages: Tensor, k_scales: Tensor, v_scales: Tensor,
+                      page_table: Tensor, seqlens: Tensor, *, max_seqlen: Optional[int] = None,
+                      scale: Optional[float] = None, chunk: int = 0) -> Tensor:
+    """Attention over an 8-bit paged cache of the newest token of each sequence (q [B, Hq, D]) or its
+    newest n (q [B, n, Hq, D], query i seeing what comes before it and itself), `seqlens` counting
+    them; the pools [num_pages, page_size, Hkv, D] are float8_e4m3fn or int8, the scales float32
+    [num_pages, page_size // block, Hkv].  See b200attn_paged_decode_8bit_fwd in include/b200attn.h."""
+    dt, block = _check_8bit_cache(k_pages, v_pages, k_scales, v_scales, page_table, q, seqlens)
+    _same_head_dim(q, k_pages)
+    if q.dtype not in _DT:
+        raise ValueError("b200attn: q must be float16 or bfloat16")
+    if q.dim() not in (3, 4) or page_table.shape[0] != q.shape[0] or seqlens.numel() != q.shape[0]:
+        raise ValueError("b200attn: q is [B, Hq, D] or [B, n, Hq, D], with B rows in page_table and seqlens")
+    o = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    if q.numel() == 0:
+        return o
+    q4, o4 = (q, o) if q.dim() == 4 else (q.unsqueeze(1), o.unsqueeze(1))
+    q4 = _rowmajor16(q4)
+    table, sl = _i32(page_table, q.device), _i32(seqlens, q.device)
+    B, n, Hq, D = q4.shape
+    P, page, Hkv, _ = k_pages.shape
+    a = PagedDecode8bitArgs()
+    a.q, a.k_pages, a.v_pages, a.o = _ptr(q4), _ptr(k_pages), _ptr(v_pages), _ptr(o)
+    a.k_scales, a.v_scales = _ptr(k_scales), _ptr(v_scales)
+    a.dtype, a.cache_dtype, a.batch, a.queries = _DT[q.dtype], dt, B, n
+    a.heads_q, a.heads_kv, a.head_dim = Hq, Hkv, D
+    a.page_size, a.block_tokens, a.num_pages, a.max_pages_per_seq = page, block, P, table.shape[1]
+    cap = min(table.shape[1] * page, 2 ** 31 - 1)
+    a.max_seqlen = cap if max_seqlen is None else min(int(max_seqlen), cap)
+    a.page_table, a.seqlens = _ptr(table), _ptr(sl)
+    a.q_stride_b, a.q_stride_t, a.q_stride_h = q4.stride()[:3]
+    a.o_stride_b, a.o_stride_t, a.o_stride_h = o4.stride()[:3]
+    _pool_strides(a, k_pages, v_pages, k_scales, v_scales)
+    a.softmax_scale = float(scale) if scale is not None else D ** -0.5
+    a.chunk_tokens = int(chunk)
+    L = _lib.lib()
+    ws = torch.empty(max(L.b200attn_paged_decode_8bit_workspace_bytes(C.byref(a)), 16), device=q.device,
+                     dtype=torch.uint8)
+    a.workspace, a.workspace_bytes = _ptr(ws), ws.numel()
+    with torch.cuda.device(q.device):
+        if DEBUG_STATUS:
+            a.status_word = _ptr(_status_word(q.device))
+        _lib.check(L.b200attn_paged_decode_8bit_fwd(C.byref(a), _stream(q)))
+        _check_status(q.device, "decoding over an 8-bit cache")
+    _count()
+    return o
+
+
+def append_kv_8bit(k_pages: Tensor, v_pages: Tensor, k_scales: Tensor, v_scales: Tensor, new_k: Tensor,
+                   new_v: Tensor, page_table: Tensor, seqlens: Tensor, *, cu_new: Optional[Tensor] = None) -> None:
+    """In place: the new rows of each sequence, quantised, at positions seqlens[b] on.  new_k, new_v
+    [B, Hkv, D] hold one row for each sequence, or [T, Hkv, D] (or [1, T, Hkv, D]) those that
+    cu_new int32 [B + 1] delimits.  See b200attn_kv_append_8bit in include/b200attn.h."""
+    dt, block = _check_8bit_cache(k_pages, v_pages, k_scales, v_scales, page_table, new_k, new_v, seqlens, cu_new)
+    if new_k.dtype not in _DT or new_v.dtype != new_k.dtype:
+        raise ValueError("b200attn: new rows must be float16 or bfloat16, K and V alike")
+    if cu_new is not None and new_k.dim() == 4 and new_k.shape[0] == 1 and new_v.dim() == 4 and new_v.shape[0] == 1:
+        new_k, new_v = new_k[0], new_v[0]
+    B = page_table.shape[0]
+    if new_k.dim() != 3 or new_v.shape != new_k.shape or new_k.shape[1:] != k_pages.shape[2:]:
+        raise ValueError("b200attn: new rows are [tokens, Hkv, D] with the pools' heads, K and V alike")
+    if seqlens.numel() != B or (cu_new is None and new_k.shape[0] != B) or (cu_new is not None and cu_new.numel() != B + 1):
+        raise ValueError("b200attn: page_table, seqlens and cu_new (or the new rows) disagree on the batch")
+    if new_k.numel() == 0:
+        return
+    nk, nv = _rowmajor16(new_k), _rowmajor16(new_v)
+    dev = k_pages.device
+    table, sl, cu = _i32(page_table, dev), _i32(seqlens, dev), _i32(cu_new, dev)
+    a = KvAppend8bitArgs()
+    a.new_k, a.new_v, a.k_pages, a.v_pages = _ptr(nk), _ptr(nv), _ptr(k_pages), _ptr(v_pages)
+    a.k_scales, a.v_scales = _ptr(k_scales), _ptr(v_scales)
+    a.dtype, a.cache_dtype, a.batch, a.heads, a.head_dim = _DT[nk.dtype], dt, B, nk.shape[1], nk.shape[2]
+    a.tokens, a.page_size, a.block_tokens = nk.shape[0], k_pages.shape[1], block
+    a.num_pages, a.max_pages_per_seq = k_pages.shape[0], table.shape[1]
+    a.page_table, a.seqlens, a.cu_new = _ptr(table), _ptr(sl), _ptr(cu)
+    a.nk_stride_t, a.nk_stride_h = nk.stride()[:2]
+    a.nv_stride_t, a.nv_stride_h = nv.stride()[:2]
+    _pool_strides(a, k_pages, v_pages, k_scales, v_scales)
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().b200attn_kv_append_8bit(C.byref(a), _stream(k_pages)))
+    _count()
+
+
+# --------------------------------------------------------------------------
+# pages of a cache (16-bit or 8-bit)
+# --------------------------------------------------------------------------
+def _book(name: str, page_table: Tensor, page_refs: Tensor, **per_slot: Tensor):
+    """The bookkeeping tensors of a cache as the kernels take them."""
+    tensors = dict(page_table=page_table, page_refs=page_refs, **per_slot)
+    _need_cuda(*tensors.values())
+    for k, t in tensors.items():
+        if t.dtype != torch.int32 or t.device != page_table.device:
+            raise ValueError(f"b200attn: {name} takes int32 tensors of one device ({k})")
+    if page_table.dim() != 2 or page_refs.dim() != 1:
+        raise ValueError(f"b200attn: {name} takes page_table [slots, max_pages] and page_refs [num_pages]")
+    for k, t in per_slot.items():
+        if t.numel() != page_table.shape[0]:
+            raise ValueError(f"b200attn: {name} takes one entry of {k} for each slot")
+    return [t.contiguous() for t in tensors.values()]
+
+
+def _page_pools(name: str, pools, page_refs: Tensor):
+    """b200attn_page_pool entries for tensors [num_pages, ...] whose pages are contiguous."""
+    pools = list(pools)
+    out = (PagePool * max(len(pools), 1))()
+    for i, t in enumerate(pools):
+        _need_cuda(t)
+        if t.device != page_refs.device or t.dim() < 1 or t.shape[0] != page_refs.numel():
+            raise ValueError(f"b200attn: {name} takes pools [num_pages, ...] on the device of page_refs")
+        page = t[0]
+        size = page.numel() * t.element_size()
+        if not page.is_contiguous() or size == 0 or size % 4 != 0 or t.data_ptr() % 4 != 0 \
+                or (t.stride(0) * t.element_size()) % 4 != 0 or (t.shape[0] > 1 and t.stride(0) < page.numel()):
+            raise ValueError(f"b200attn: {name} takes pools whose pages are contiguous, apart and multiples of 4 bytes")
+        out[i] = PagePool(t.data_ptr(), size, max(t.stride(0) * t.element_size(), size))
+    return pools, out
+
+
+def _run_pages(a, fn: str, like: Tensor):
+    L = _lib.lib()
+    ws = torch.empty(max(getattr(L, fn + "_workspace_bytes")(C.byref(a)), 16), device=like.device, dtype=torch.uint8)
+    a.workspace, a.workspace_bytes = _ptr(ws), ws.numel()
+    with torch.cuda.device(like.device):
+        _lib.check(getattr(L, fn)(C.byref(a), _stream(like)))
+    _count()
+
+
+def grow_pages(page_table: Tensor, seqlens: Tensor, page_refs: Tensor, new_tokens: Tensor, *,
+               page_size: int) -> Tuple[Tensor, Tensor, Tensor]:
+    """Pages for the new_tokens int32 [slots] to come: (page_table, page_refs, missing int32 [1]), new
+    tensors; `missing` counts pages that could not be given.  See b200attn_pages_grow in
+    include/b200attn.h."""
+    table, refs, lens, new = _book("grow_pages", page_table, page_refs, seqlens=seqlens, new_tokens=new_tokens)
+    out, refs_out = torch.empty_like(table), torch.empty_like(refs)
+    missing = torch.empty(1, device=refs.device, dtype=torch.int32)
+    a = PagesGrowArgs(_ptr(table), _ptr(lens), _ptr(refs), _ptr(new), _ptr(out), _ptr(refs_out), _ptr(missing),
+                      table.shape[0], table.shape[1], refs.numel(), int(page_size))
+    _run_pages(a, "b200attn_pages_grow", table)
+    return out, refs_out, missing
+
+
+def fork_pages(pools, page_table: Tensor, seqlens: Tensor, page_refs: Tensor, parents: Tensor, *,
+               page_size: int) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
+    """Every slot b becomes the sequence of slot parents[b] (int32 [slots]; outside [0, slots): freed):
+    (page_table, seqlens, page_refs, missing int32 [1]), new tensors.  Full pages are shared; partly
+    filled last ones are copied in every tensor of `pools` ([num_pages, ...]: the K and V pools of
+    all layers, and their scales).  See b200attn_pages_fork in include/b200attn.h."""
+    table, refs, lens, par = _book("fork_pages", page_table, page_refs, seqlens=seqlens, parents=parents)
+    pools, entries = _page_pools("fork_pages", pools, refs)
+    out, lens_out, refs_out = torch.empty_like(table), torch.empty_like(lens), torch.empty_like(refs)
+    missing = torch.empty(1, device=refs.device, dtype=torch.int32)
+    a = PagesForkArgs(_ptr(table), _ptr(lens), _ptr(refs), _ptr(par), _ptr(out), _ptr(lens_out), _ptr(refs_out),
+                      _ptr(missing), entries, len(pools), table.shape[0], table.shape[1], refs.numel(), int(page_size))
+    _run_pages(a, "b200attn_pages_fork", table)
+    return out, lens_out, refs_out, missing
+
+
+def compact_pages(pools, page_table: Tensor, page_refs: Tensor) -> Tuple[Tensor, Tensor, Tensor]:
+    """The pages in use moved to the front of every tensor of `pools` ([num_pages, ...]):
+    (page_table, page_refs, live int32 [1]), new tensors; `live` is the number of pages in use.  See
+    b200attn_pages_compact in include/b200attn.h."""
+    table, refs = _book("compact_pages", page_table, page_refs)
+    pools, entries = _page_pools("compact_pages", pools, refs)
+    out, refs_out = torch.empty_like(table), torch.empty_like(refs)
+    live = torch.empty(1, device=refs.device, dtype=torch.int32)
+    a = PagesCompactArgs(_ptr(table), _ptr(refs), _ptr(out), _ptr(refs_out), _ptr(live), entries, len(pools),
+                         table.shape[0], table.shape[1], refs.numel())
+    _run_pages(a, "b200attn_pages_compact", table)
+    return out, refs_out, live
 
 
 # --------------------------------------------------------------------------
