@@ -546,3 +546,48 @@ def test_refusals():
     with pytest.raises(RuntimeError, match="CUDA tensors only"):
         ops.paged_decode_8bit(q.cpu(), k, v, ks, vs, t, n)
     assert ops.paged_decode_8bit(q[:0], k, v, ks, vs, t[:0], n[:0]).shape == (0, 4, 64)
+
+
+def test_native_calls_equal_python_calls(monkeypatch):
+    """Same bits from the native call path and the Python one, and who answered."""
+    from tritonops_b200 import ops
+    lens = torch.tensor([300, 17, 0], dtype=i32)
+    table, pages = rows_of(56, [n + 40 for n in lens.tolist()], 32)
+    host = cache(57, pages, 32, 16, 2, 64, I8)
+    g = torch.Generator().manual_seed(58)
+    q, rows = torch.randn(3, 2, 8, 64, generator=g).half().cuda(), torch.randn(2, 9, 2, 64, generator=g).half().cuda()
+    t, n, cu = table.cuda(), lens.cuda(), torch.tensor([0, 4, 4, 9], dtype=i32).cuda()
+    refs = torch.zeros(pages, dtype=i32)
+    refs[table[table >= 0].long()] = 1
+    refs, par, new = refs.cuda(), torch.tensor([0, 0, 2], dtype=i32).cuda(), torch.tensor([50, 0, 3], dtype=i32).cuda()
+
+    def results():
+        dev = [p.cuda() for p in host]
+        out = [ops.paged_decode_8bit(q, *dev, t, n), ops.paged_decode_8bit(q[:, 0], *dev, t, n, max_seqlen=200, scale=0.3),
+               ops.paged_decode_8bit(q[:, 1], *dev, t.long(), n, chunk=128),          # left to Python
+               ops.paged_decode_8bit(q[..., 1:].contiguous()[..., :32], *(p[..., :32] if p.dim() == 4 else p for p in dev),
+                                     t, n)]                                           # rows off 16 bytes: Python
+        ops.append_kv_8bit(*dev, rows[0], rows[1], t, n, cu_new=cu)
+        ops.append_kv_8bit(*dev, rows[0][:3], rows[1][:3], t, n + 20)
+        ops.append_kv_8bit(*dev, rows[0][None], rows[1][None], t, n, cu_new=cu)       # left to Python
+        out += [*ops.grow_pages(t, n, refs, new, page_size=32), *ops.fork_pages(dev, t, n, refs, par, page_size=32),
+                *ops.fork_pages(iter(dev), t, n, refs, par, page_size=32),            # left to Python
+                *ops.compact_pages(tuple(dev), t, refs)]
+        return [bits(x).cpu() for x in out + dev]
+
+    real, answered = ops._native, []
+
+    def spy(name, *args):
+        r = real(name, *args)
+        answered.append((name, r is not None))
+        return r
+
+    monkeypatch.setattr(ops, "_native", spy)
+    native = results()
+    decode = [a for name, a in answered if name == "paged_decode_8bit"]
+    assert decode == [True, True, False, False]
+    assert [a for name, a in answered if name == "append_kv_8bit"] == [True, True, False]
+    assert [a for name, a in answered if name.endswith("_pages")] == [True, True, False, True]
+    monkeypatch.setattr(ops, "_native", lambda *a: None)
+    for i, (a, b) in enumerate(zip(native, results())):
+        assert same_bits(a, b), i

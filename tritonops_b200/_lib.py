@@ -219,7 +219,7 @@ NOALLOC_SCRATCH_BYTES = 32 << 20
 
 # the argument structs csrc/host.cpp fills, in the order its init() takes their sizes
 HOST_STRUCTS = (PrefillArgs, PrefillBwdArgs, DecodeArgs, PagedDecodeArgs, KvAppendArgs, TopkBlocksArgs, RmsNormFwdArgs,
-                RmsNormBwdArgs)
+                RmsNormBwdArgs, PagedDecode8bitArgs, KvAppend8bitArgs, PagesGrowArgs, PagesForkArgs, PagesCompactArgs)
 
 _lib = None
 _host = None

@@ -20,6 +20,7 @@
 
 #include <algorithm>
 #include <exception>
+#include <vector>
 
 #include "../../include/b200attn.h"
 
@@ -37,6 +38,15 @@ struct Lib {
   decltype(&b200attn_paged_decode_fwd) paged_decode_fwd;
   decltype(&b200attn_kv_append) kv_append;
   decltype(&b200attn_topk_blocks) topk_blocks;
+  decltype(&b200attn_paged_decode_8bit_workspace_bytes) paged_decode_8bit_workspace_bytes;
+  decltype(&b200attn_paged_decode_8bit_fwd) paged_decode_8bit_fwd;
+  decltype(&b200attn_kv_append_8bit) kv_append_8bit;
+  decltype(&b200attn_pages_grow_workspace_bytes) pages_grow_workspace_bytes;
+  decltype(&b200attn_pages_grow) pages_grow;
+  decltype(&b200attn_pages_fork_workspace_bytes) pages_fork_workspace_bytes;
+  decltype(&b200attn_pages_fork) pages_fork;
+  decltype(&b200attn_pages_compact_workspace_bytes) pages_compact_workspace_bytes;
+  decltype(&b200attn_pages_compact) pages_compact;
   decltype(&b200attn_rmsnorm_fwd) rmsnorm_fwd;
   decltype(&b200attn_rmsnorm_bwd_workspace_bytes) rmsnorm_bwd_workspace_bytes;
   decltype(&b200attn_rmsnorm_bwd) rmsnorm_bwd;
@@ -326,6 +336,192 @@ PyObject* append_kv(PyObject*, PyObject* const* x, Py_ssize_t n) {
   });
 }
 
+// The pools, scales and page table of an 8-bit cache, in the layout the kernels take, into `a`.
+template <typename A>
+void cache_8bit(A& a, const at::Tensor& k, const at::Tensor& v, const at::Tensor& ks, const at::Tensor& vs, PyObject* table_,
+                at::Tensor& table) {
+  const auto type = k.scalar_type();
+  need((type == at::kFloat8_e4m3fn || type == at::kChar) && v.scalar_type() == type);
+  need(k.dim() == 4 && v.sizes() == k.sizes() && ks.dim() == 3 && vs.sizes() == ks.sizes());
+  need(ks.scalar_type() == at::kFloat && vs.scalar_type() == at::kFloat);
+  for (const at::Tensor* t : {&v, &ks, &vs}) need(t->device() == k.device());
+  for (const at::Tensor* t : {&k, &v}) need(t->stride(3) == 1);
+  need(k.numel() > 0 && k.size(0) <= INT32_MAX && k.size(1) <= INT32_MAX && k.size(2) <= INT32_MAX);
+  need(ks.size(0) == k.size(0) && ks.size(2) == k.size(2) && ks.size(1) > 0 && k.size(1) % ks.size(1) == 0);
+  need(table_ != Py_None);
+  a.page_table = int_list(table_, k, &table);
+  need(table.dim() == 2 && table.size(0) <= INT32_MAX && table.size(1) <= INT32_MAX);
+  a.cache_dtype = type == at::kChar ? B200ATTN_I8 : B200ATTN_E4M3;
+  a.k_pages = k.data_ptr(); a.v_pages = v.data_ptr();
+  a.k_scales = ks.data_ptr<float>(); a.v_scales = vs.data_ptr<float>();
+  a.num_pages = (int)k.size(0); a.page_size = (int)k.size(1);
+  a.block_tokens = (int)(k.size(1) / ks.size(1)); a.max_pages_per_seq = (int)table.size(1);
+  a.k_stride_page = k.stride(0); a.k_stride_t = k.stride(1); a.k_stride_h = k.stride(2);
+  a.v_stride_page = v.stride(0); a.v_stride_t = v.stride(1); a.v_stride_h = v.stride(2);
+  a.ks_stride_page = ks.stride(0); a.ks_stride_blk = ks.stride(1); a.ks_stride_h = ks.stride(2);
+  a.vs_stride_page = vs.stride(0); a.vs_stride_blk = vs.stride(1); a.vs_stride_h = vs.stride(2);
+}
+
+// q, k_pages, v_pages, k_scales, v_scales, page_table, seqlens, max_seqlen | None, scale | None, chunk
+PyObject* paged_decode_8bit(PyObject*, PyObject* const* x, Py_ssize_t n) {
+  return guarded(n, 10, [&]() -> PyObject* {
+    const at::Tensor &q = tensor(x[0]), &k = tensor(x[1]), &v = tensor(x[2]), &ks = tensor(x[3]), &vs = tensor(x[4]);
+    const int64_t dim = q.dim();
+    need((dim == 3 || dim == 4) && q.numel() > 0);
+    row_major(q, q, dim);
+    b200attn_paged_decode_8bit_args a = {};
+    at::Tensor table, lens;
+    cache_8bit(a, k, v, ks, vs, x[5], table);
+    need(x[6] != Py_None && k.device() == q.device() && k.size(3) == q.size(dim - 1));
+    a.seqlens = int_list(x[6], q, &lens);
+    need(table.size(0) == q.size(0) && lens.numel() == q.size(0) && q.numel() <= INT32_MAX);
+    a.dtype = dtype16(q);
+    a.batch = (int)q.size(0); a.queries = dim == 4 ? (int)q.size(1) : 1;
+    a.heads_q = (int)q.size(dim - 2); a.heads_kv = (int)k.size(2); a.head_dim = (int)q.size(dim - 1);
+    const long long cap = std::min<long long>(table.size(1) * k.size(1), INT32_MAX);
+    a.max_seqlen = x[7] == Py_None ? (int)cap : (int)std::min<long long>(integer(x[7]), cap);
+    a.softmax_scale = x[8] == Py_None ? (float)std::pow((double)a.head_dim, -0.5) : real(x[8]);
+    a.chunk_tokens = int32(x[9]);
+    const c10::cuda::CUDAGuard device(q.device());
+    at::Tensor o = fresh(q.sizes(), q);
+    a.q = q.data_ptr(); a.o = o.data_ptr();
+    a.q_stride_b = q.stride(0); a.q_stride_t = dim == 4 ? q.stride(1) : 0; a.q_stride_h = q.stride(dim - 2);
+    a.o_stride_b = o.stride(0); a.o_stride_t = dim == 4 ? o.stride(1) : 0; a.o_stride_h = o.stride(dim - 2);
+    at::Tensor ws = scratch(L.paged_decode_8bit_workspace_bytes(&a), q);
+    a.workspace = ws.data_ptr(); a.workspace_bytes = (size_t)ws.numel();
+    long long launches;
+    const int st = call(L.paged_decode_8bit_fwd, a, q, launches);
+    return answer(st, launches, {o});
+  });
+}
+
+// k_pages, v_pages, k_scales, v_scales, new_k, new_v, page_table, seqlens, cu_new | None
+PyObject* append_kv_8bit(PyObject*, PyObject* const* x, Py_ssize_t n) {
+  return guarded(n, 9, [&]() -> PyObject* {
+    const at::Tensor &k = tensor(x[0]), &v = tensor(x[1]), &ks = tensor(x[2]), &vs = tensor(x[3]), &nk = tensor(x[4]),
+                     &nv = tensor(x[5]);
+    row_major(nk, nk, 3); row_major(nv, nk, 3);
+    b200attn_kv_append_8bit_args a = {};
+    at::Tensor table, lens, cu;
+    cache_8bit(a, k, v, ks, vs, x[6], table);
+    need(nk.device() == k.device() && nk.numel() > 0 && nv.sizes() == nk.sizes());
+    need(nk.size(1) == k.size(2) && nk.size(2) == k.size(3) && x[7] != Py_None);
+    a.seqlens = int_list(x[7], k, &lens); a.cu_new = int_list(x[8], k, &cu);
+    need(lens.numel() == table.size(0) && (a.cu_new ? cu.numel() == table.size(0) + 1 : nk.size(0) == table.size(0)));
+    a.dtype = dtype16(nk);
+    a.batch = (int)table.size(0); a.heads = (int)nk.size(1); a.head_dim = (int)nk.size(2); a.tokens = nk.size(0);
+    a.new_k = nk.data_ptr(); a.new_v = nv.data_ptr();
+    a.nk_stride_t = nk.stride(0); a.nk_stride_h = nk.stride(1);
+    a.nv_stride_t = nv.stride(0); a.nv_stride_h = nv.stride(1);
+    const c10::cuda::CUDAGuard device(k.device());
+    long long launches;
+    const int st = call(L.kv_append_8bit, a, k, launches);
+    return answer(st, launches, {});
+  });
+}
+
+// page_table and page_refs of the page operators; their other int32 tensors have an entry per slot
+template <typename A>
+void book(A& a, PyObject* table_, PyObject* refs_, at::Tensor& table, at::Tensor& refs) {
+  table = tensor(table_);
+  a.page_table = int_list(table_, table); a.page_refs = int_list(refs_, table, &refs);
+  need(a.page_table && a.page_refs && table.dim() == 2 && refs.dim() == 1);
+  need(table.size(0) <= INT32_MAX && table.size(1) <= INT32_MAX && refs.numel() <= INT32_MAX);
+  a.slots = (int)table.size(0); a.max_pages_per_seq = (int)table.size(1); a.num_pages = (int)refs.numel();
+}
+const int32_t* per_slot(PyObject* o, const at::Tensor& table, at::Tensor& t) {
+  const int32_t* p = int_list(o, table, &t);
+  need(p && t.numel() == table.size(0));
+  return p;
+}
+at::Tensor one_int(const at::Tensor& like) { return at::empty({1}, like.options().requires_grad(false)); }
+
+// tensors [num_pages, ...] whose pages are contiguous
+std::vector<b200attn_page_pool> page_pools(PyObject* list, const at::Tensor& refs) {
+  need(PyList_CheckExact(list) || PyTuple_CheckExact(list));
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(list);
+  need(n <= INT32_MAX);
+  std::vector<b200attn_page_pool> out;
+  out.reserve((size_t)n);
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    const at::Tensor& t = tensor(PySequence_Fast_GET_ITEM(list, i));
+    need(t.device() == refs.device() && t.dim() >= 1 && t.size(0) == refs.numel() && t.numel() > 0);
+    int64_t each = 1;      // numbers of a page, contiguous
+    for (int64_t d = t.dim() - 1; d > 0; --d) {
+      need(t.size(d) == 1 || t.stride(d) == each);
+      each *= t.size(d);
+    }
+    const int64_t size = (int64_t)t.element_size(), bytes = each * size;
+    need(bytes % 4 == 0 && (uintptr_t)t.data_ptr() % 4 == 0 && t.stride(0) * size % 4 == 0);
+    need(t.size(0) == 1 || t.stride(0) >= each);
+    out.push_back({t.data_ptr(), bytes, std::max(t.stride(0) * size, bytes)});
+  }
+  return out;
+}
+
+// page_table, seqlens, page_refs, new_tokens, page_size
+PyObject* grow_pages(PyObject*, PyObject* const* x, Py_ssize_t n) {
+  return guarded(n, 5, [&]() -> PyObject* {
+    b200attn_pages_grow_args a = {};
+    at::Tensor table, refs, lens, more;
+    book(a, x[0], x[2], table, refs);
+    a.seqlens = per_slot(x[1], table, lens); a.new_tokens = per_slot(x[3], table, more);
+    a.page_size = int32(x[4]);
+    const c10::cuda::CUDAGuard device(table.device());
+    at::Tensor out = fresh(table.sizes(), table), refs_out = fresh(refs.sizes(), refs), missing = one_int(refs);
+    a.page_table_out = out.data_ptr<int32_t>(); a.page_refs_out = refs_out.data_ptr<int32_t>();
+    a.missing_out = missing.data_ptr<int32_t>();
+    at::Tensor ws = scratch(L.pages_grow_workspace_bytes(&a), table);
+    a.workspace = ws.data_ptr(); a.workspace_bytes = (size_t)ws.numel();
+    long long launches;
+    const int st = call(L.pages_grow, a, table, launches);
+    return answer(st, launches, {out, refs_out, missing});
+  });
+}
+
+// pools, page_table, seqlens, page_refs, parents, page_size
+PyObject* fork_pages(PyObject*, PyObject* const* x, Py_ssize_t n) {
+  return guarded(n, 6, [&]() -> PyObject* {
+    b200attn_pages_fork_args a = {};
+    at::Tensor table, refs, lens, parents;
+    book(a, x[1], x[3], table, refs);
+    a.seqlens = per_slot(x[2], table, lens); a.parents = per_slot(x[4], table, parents);
+    a.page_size = int32(x[5]);
+    const std::vector<b200attn_page_pool> pools = page_pools(x[0], refs);
+    a.pools = pools.data(); a.n_pools = (int)pools.size();
+    const c10::cuda::CUDAGuard device(table.device());
+    at::Tensor out = fresh(table.sizes(), table), refs_out = fresh(refs.sizes(), refs), missing = one_int(refs),
+               lens_out = fresh(lens.sizes(), lens);
+    a.page_table_out = out.data_ptr<int32_t>(); a.page_refs_out = refs_out.data_ptr<int32_t>();
+    a.seqlens_out = lens_out.data_ptr<int32_t>(); a.missing_out = missing.data_ptr<int32_t>();
+    at::Tensor ws = scratch(L.pages_fork_workspace_bytes(&a), table);
+    a.workspace = ws.data_ptr(); a.workspace_bytes = (size_t)ws.numel();
+    long long launches;
+    const int st = call(L.pages_fork, a, table, launches);
+    return answer(st, launches, {out, lens_out, refs_out, missing});
+  });
+}
+
+// pools, page_table, page_refs
+PyObject* compact_pages(PyObject*, PyObject* const* x, Py_ssize_t n) {
+  return guarded(n, 3, [&]() -> PyObject* {
+    b200attn_pages_compact_args a = {};
+    at::Tensor table, refs;
+    book(a, x[1], x[2], table, refs);
+    const std::vector<b200attn_page_pool> pools = page_pools(x[0], refs);
+    a.pools = pools.data(); a.n_pools = (int)pools.size();
+    const c10::cuda::CUDAGuard device(table.device());
+    at::Tensor out = fresh(table.sizes(), table), refs_out = fresh(refs.sizes(), refs), live = one_int(refs);
+    a.page_table_out = out.data_ptr<int32_t>(); a.page_refs_out = refs_out.data_ptr<int32_t>();
+    a.live_out = live.data_ptr<int32_t>();
+    at::Tensor ws = scratch(L.pages_compact_workspace_bytes(&a), table);
+    a.workspace = ws.data_ptr(); a.workspace_bytes = (size_t)ws.numel();
+    long long launches;
+    const int st = call(L.pages_compact, a, table, launches);
+    return answer(st, launches, {out, refs_out, live});
+  });
+}
+
 // scores, top_k, n_valid | None, force_first, force_last
 PyObject* topk_blocks(PyObject*, PyObject* const* x, Py_ssize_t n) {
   return guarded(n, 5, [&]() -> PyObject* {
@@ -429,7 +625,9 @@ PyObject* init(PyObject*, PyObject* const* x, Py_ssize_t n) {
   const size_t sizes[] = {sizeof(b200attn_prefill_args), sizeof(b200attn_prefill_bwd_args), sizeof(b200attn_decode_args),
                           sizeof(b200attn_paged_decode_args), sizeof(b200attn_kv_append_args),
                           sizeof(b200attn_topk_blocks_args), sizeof(b200attn_rmsnorm_fwd_args),
-                          sizeof(b200attn_rmsnorm_bwd_args)};
+                          sizeof(b200attn_rmsnorm_bwd_args), sizeof(b200attn_paged_decode_8bit_args),
+                          sizeof(b200attn_kv_append_8bit_args), sizeof(b200attn_pages_grow_args),
+                          sizeof(b200attn_pages_fork_args), sizeof(b200attn_pages_compact_args)};
   constexpr Py_ssize_t kStructs = sizeof(sizes) / sizeof(sizes[0]);
   bool same = n == 1 + kStructs;
   for (Py_ssize_t i = 0; same && i < kStructs; ++i) same = PyLong_AsSize_t(x[1 + i]) == sizes[i];
@@ -448,7 +646,12 @@ PyObject* init(PyObject*, PyObject* const* x, Py_ssize_t n) {
         B(decode_fwd, decode_fwd) && B(sparse_decode_fwd, sparse_decode_fwd) &&
         B(paged_decode_workspace_bytes, paged_decode_workspace_bytes) && B(paged_decode_fwd, paged_decode_fwd) &&
         B(kv_append, kv_append) && B(topk_blocks, topk_blocks) && B(rmsnorm_fwd, rmsnorm_fwd) &&
-        B(rmsnorm_bwd_workspace_bytes, rmsnorm_bwd_workspace_bytes) && B(rmsnorm_bwd, rmsnorm_bwd)))
+        B(rmsnorm_bwd_workspace_bytes, rmsnorm_bwd_workspace_bytes) && B(rmsnorm_bwd, rmsnorm_bwd) &&
+        B(paged_decode_8bit_workspace_bytes, paged_decode_8bit_workspace_bytes) &&
+        B(paged_decode_8bit_fwd, paged_decode_8bit_fwd) && B(kv_append_8bit, kv_append_8bit) &&
+        B(pages_grow_workspace_bytes, pages_grow_workspace_bytes) && B(pages_grow, pages_grow) &&
+        B(pages_fork_workspace_bytes, pages_fork_workspace_bytes) && B(pages_fork, pages_fork) &&
+        B(pages_compact_workspace_bytes, pages_compact_workspace_bytes) && B(pages_compact, pages_compact)))
     return nullptr;
 #undef B
   ready = true;
@@ -457,7 +660,8 @@ PyObject* init(PyObject*, PyObject* const* x, Py_ssize_t n) {
 
 #define FAST(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(prefill), FAST(prefill_bwd), FAST(decode), FAST(paged_decode), FAST(append_kv),
-                         FAST(topk_blocks), FAST(rmsnorm_fwd), FAST(rmsnorm_bwd),
+                         FAST(topk_blocks), FAST(rmsnorm_fwd), FAST(rmsnorm_bwd), FAST(paged_decode_8bit),
+                         FAST(append_kv_8bit), FAST(grow_pages), FAST(fork_pages), FAST(compact_pages),
                          FAST(init), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_b200host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -622,6 +622,10 @@ def paged_decode_8bit(q: Tensor, k_pages: Tensor, v_pages: Tensor, k_scales: Ten
     newest n (q [B, n, Hq, D], query i seeing what comes before it and itself), `seqlens` counting
     them; the pools [num_pages, page_size, Hkv, D] are float8_e4m3fn or int8, the scales float32
     [num_pages, page_size // block, Hkv].  See b200attn_paged_decode_8bit_fwd in include/b200attn.h."""
+    r = _native("paged_decode_8bit", q, k_pages, v_pages, k_scales, v_scales, page_table, seqlens, max_seqlen, scale,
+                chunk)
+    if r is not None:
+        return r[0]
     dt, block = _check_8bit_cache(k_pages, v_pages, k_scales, v_scales, page_table, q, seqlens)
     _same_head_dim(q, k_pages)
     if q.dtype not in _DT:
@@ -668,6 +672,9 @@ def append_kv_8bit(k_pages: Tensor, v_pages: Tensor, k_scales: Tensor, v_scales:
     """In place: the new rows of each sequence, quantised, at positions seqlens[b] on.  new_k, new_v
     [B, Hkv, D] hold one row for each sequence, or [T, Hkv, D] (or [1, T, Hkv, D]) those that
     cu_new int32 [B + 1] delimits.  See b200attn_kv_append_8bit in include/b200attn.h."""
+    if _native("append_kv_8bit", k_pages, v_pages, k_scales, v_scales, new_k, new_v, page_table, seqlens,
+               cu_new) is not None:
+        return
     dt, block = _check_8bit_cache(k_pages, v_pages, k_scales, v_scales, page_table, new_k, new_v, seqlens, cu_new)
     if new_k.dtype not in _DT or new_v.dtype != new_k.dtype:
         raise ValueError("b200attn: new rows must be float16 or bfloat16, K and V alike")
@@ -747,6 +754,9 @@ def grow_pages(page_table: Tensor, seqlens: Tensor, page_refs: Tensor, new_token
     """Pages for the new_tokens int32 [slots] to come: (page_table, page_refs, missing int32 [1]), new
     tensors; `missing` counts pages that could not be given.  See b200attn_pages_grow in
     include/b200attn.h."""
+    r = _native("grow_pages", page_table, seqlens, page_refs, new_tokens, page_size)
+    if r is not None:
+        return r
     table, refs, lens, new = _book("grow_pages", page_table, page_refs, seqlens=seqlens, new_tokens=new_tokens)
     out, refs_out = torch.empty_like(table), torch.empty_like(refs)
     missing = torch.empty(1, device=refs.device, dtype=torch.int32)
@@ -762,6 +772,9 @@ def fork_pages(pools, page_table: Tensor, seqlens: Tensor, page_refs: Tensor, pa
     (page_table, seqlens, page_refs, missing int32 [1]), new tensors.  Full pages are shared; partly
     filled last ones are copied in every tensor of `pools` ([num_pages, ...]: the K and V pools of
     all layers, and their scales).  See b200attn_pages_fork in include/b200attn.h."""
+    r = _native("fork_pages", pools, page_table, seqlens, page_refs, parents, page_size)
+    if r is not None:
+        return r
     table, refs, lens, par = _book("fork_pages", page_table, page_refs, seqlens=seqlens, parents=parents)
     pools, entries = _page_pools("fork_pages", pools, refs)
     out, lens_out, refs_out = torch.empty_like(table), torch.empty_like(lens), torch.empty_like(refs)
@@ -776,6 +789,9 @@ def compact_pages(pools, page_table: Tensor, page_refs: Tensor) -> Tuple[Tensor,
     """The pages in use moved to the front of every tensor of `pools` ([num_pages, ...]):
     (page_table, page_refs, live int32 [1]), new tensors; `live` is the number of pages in use.  See
     b200attn_pages_compact in include/b200attn.h."""
+    r = _native("compact_pages", pools, page_table, page_refs)
+    if r is not None:
+        return r
     table, refs = _book("compact_pages", page_table, page_refs)
     pools, entries = _page_pools("compact_pages", pools, refs)
     out, refs_out = torch.empty_like(table), torch.empty_like(refs)
