@@ -40,6 +40,20 @@ constexpr int kUnits = kStageKeys / kUnitKeys;
 constexpr int kRowsTile = 16;      // query rows (query x head of the group) of a work item
 constexpr float kPUp = 10.f;       // P is 2^kPUp times the weight
 
+// n / d for 0 <= n < 2^31 by a multiplication (a division by a run-time number takes the producer
+// warp longer than the copy it prepares)
+struct Divisor {
+  unsigned mul;
+  int shift, d;
+  __device__ __forceinline__ int quotient(int n) const { return (int)(((unsigned long long)(unsigned)n * mul) >> shift); }
+  __device__ __forceinline__ int remainder(int n) const { return n - quotient(n) * d; }
+};
+Divisor divisor(int d) {      // mul = ceil(2^shift / d) < 2^32, exact for n < 2^31 as 2^31 * (mul * d - 2^shift) <= 2^shift
+  int bits = 0;
+  while ((1LL << bits) < d) ++bits;
+  return {(unsigned)(((1ULL << (31 + bits)) + d - 1) / d), 31 + bits, d};
+}
+
 struct Decode8Params {
   const void* q;
   const float* ks;
@@ -54,7 +68,8 @@ struct Decode8Params {
   long long ks_sp, ks_sb, ks_sh, vs_sp, vs_sb, vs_sh;
   int batch, queries, heads_kv, group, head_dim;
   int rows, tiles;   // queries * group rows of a KV head, in tiles of 16
-  int page_size, block, num_pages, width, max_len;
+  Divisor by_page, by_group, by_tiles;
+  int block_shift, num_pages, width, max_len;
   int box_keys;      // keys of a copy: the largest power of two, up to a stage, that divides a page
   int chunk, max_chunks, take_over, direct_o;
   float scale_log2;
@@ -73,6 +88,9 @@ struct Decode8Item {
   int pad;
 };
 
+constexpr int kConsumers = kStageKeys / kWarpKeys;   // warps
+constexpr int kDecode8Threads = 32 * kConsumers + 32;
+
 template <int DP>
 struct Decode8Smem {
   static constexpr int kTileBytes = kStageKeys * DP;       // K or V of one stage
@@ -80,10 +98,8 @@ struct Decode8Smem {
   static constexpr int kStages = DP == 128 ? 3 : 6;
   static constexpr int kQ = kStages * kStageBytes;         // the item's 16 query rows, fp16
   static constexpr int kQPitch = DP * 2 + 16;              // bytes
-  static constexpr int kFold = kQ + kRowsTile * kQPitch;   // [4 warps][16 rows][32 columns] or [8][64], padded
-  static constexpr int kFoldBytes = 4 * 16 * 36 * 4;
-  static constexpr int kMl = kFold + kFoldBytes;           // row max and sum, [2][4 warps][16]
-  static constexpr int kRowScale = kMl + 2 * 4 * 16 * 4;   // [16] what the query rows were divided by
+  static constexpr int kMl = kQ + kRowsTile * kQPitch;     // row max and sum, [2][warps][16]
+  static constexpr int kRowScale = kMl + 2 * kConsumers * 16 * 4;   // [16] what the query rows were divided by
   static constexpr int kScales = kRowScale + 64;           // [stage][unit] (ks, vs)
   static constexpr int kMask = kScales + kStages * kUnits * 8;   // [stage] units whose page is in the pool
   static constexpr int kItem = kMask + 32;
@@ -91,8 +107,8 @@ struct Decode8Smem {
   static constexpr int kBarOffset = kNext + 16;
   static constexpr int kBytes = kBarOffset + (2 * kStages + 3) * 8 + 16;
   static constexpr int kAlloc = kBytes + 1024;
-  static_assert(kFold % 16 == 0 && kScales % 8 == 0 && kNext % 16 == 0 && kBarOffset % 8 == 0, "aligned");
-  static_assert(kFoldBytes >= 4 * 8 * 68 * 4, "either form of the fold");
+  static_assert(kScales % 8 == 0 && kNext % 16 == 0 && kBarOffset % 8 == 0, "aligned");
+  static_assert(kStageBytes == kConsumers * 16 * DP * 4, "the warps' sums of 16 rows fold in the buffer of a stage");
   static_assert(2 * (kAlloc + 1024) <= 228 * 1024, "two CTAs per SM");
 };
 
@@ -156,7 +172,7 @@ __device__ __forceinline__ void alternates(unsigned w, unsigned& even, unsigned&
 
 // T: the type of q and o.  kRows: 8 or 16 query rows are in use.
 template <typename T, bool kE4M3, int DP, int kRows>
-__global__ void __launch_bounds__(160, 2)
+__global__ void __launch_bounds__(kDecode8Threads, 2)
 decode_8bit_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                    const Decode8Params p) {
   using L = Decode8Smem<DP>;
@@ -181,14 +197,14 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
   launch_dependents();
   if (threadIdx.x == 0) {
     *abort_flag = 0;
-    for (int s = 0; s < L::kStages; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 4); }
+    for (int s = 0; s < L::kStages; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), kConsumers); }
     mbar_init(item_full, 1);
-    mbar_init(item_empty, 4);
+    mbar_init(item_empty, kConsumers);
     mbar_init(next_full, 1);
     fence_barrier_init();
     fence_proxy_async();
   }
-  if (threadIdx.x == 128) { prefetch_tmap(&tmap_k); prefetch_tmap(&tmap_v); }
+  if (threadIdx.x == 32 * kConsumers) { prefetch_tmap(&tmap_k); prefetch_tmap(&tmap_v); }
   grid_dependency_wait();
   __syncthreads();
 
@@ -197,53 +213,80 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
     const bool done = mbar_wait(bar, parity, abort_flag);
     return __all_sync(0xffffffffu, done);
   };
-  if (warp == 4) {
+  if (warp == kConsumers) {
     // ================================================================ producer
-    int x = blockIdx.x, b = blockIdx.y, chunk_id = blockIdx.z;
+    // Everything small that a copy needs is asked for long before it: behind a full ring (two CTAs'
+    // 192 KB per SM) a load takes as long as those bytes take to arrive, 3 to 4 us.  So nothing below
+    // computes with a loaded value until stages later: a batch of units' page-table entries are asked
+    // for two batches ahead and its scales one, the next item while this one's last eight stages leave.
+    constexpr int kVec = DP / 8;        // 16-byte pieces of a query row
+    constexpr int kQRows = 8 * kNT;
+    constexpr int kBatch = 32 * kUnitKeys;   // keys of a batch of units, one per lane: four stages
+    struct Head {
+      int x, b, chunk_id;
+      int len;                          // as it stands in memory
+      int entry, entry_nx;              // page-table entries of the lane's units of the first two batches
+      float2 sc;                        // scales of its unit of the first one
+      uint4 q[kQRows * kVec / 32];
+    };
+    auto fetch = [&](Head& h) {
+      const int32_t* pages = p.table + (long long)h.b * p.width;
+      const int t = h.chunk_id * p.chunk + kUnitKeys * lane;      // (the row has an entry there, if perhaps not a page)
+      h.entry = h.entry_nx = -1;
+      if (t < p.max_len) h.entry = pages[p.by_page.quotient(t)];
+      if (t + kBatch < p.max_len) h.entry_nx = pages[p.by_page.quotient(t + kBatch)];
+      h.len = p.lens[h.b];
+      const int hk = p.by_tiles.quotient(h.x), row0 = p.by_tiles.remainder(h.x) * kRowsTile;
+#pragma unroll
+      for (int i = 0; i < kQRows * kVec / 32; ++i) {
+        const int r = row0 + (lane + 32 * i) / kVec, c = (lane + 32 * i) % kVec;
+        h.q[i] = make_uint4(0, 0, 0, 0);
+        if (r < p.rows && 8 * c < p.head_dim)
+          h.q[i] = *reinterpret_cast<const uint4*>((const T*)p.q + h.b * p.q_sb + p.by_group.quotient(r) * p.q_st +
+                                                   (hk * p.group + p.by_group.remainder(r)) * p.q_sh + 8 * c);
+      }
+    };
+    // scales of the unit at key t, whose page-table entry is e (whether or not the sequence has that key)
+    auto scales_of = [&](int hk, int t, int e) -> float2 {
+      float2 r = make_float2(0.f, 0.f);
+      if (e >= 0 && e < p.num_pages) {
+        const int blk = p.by_page.remainder(t) >> p.block_shift;
+        r.x = p.ks[e * p.ks_sp + blk * p.ks_sb + hk * p.ks_sh];
+        r.y = p.vs[e * p.vs_sp + blk * p.vs_sb + hk * p.vs_sh];
+      }
+      return r;
+    };
+    auto first_scales = [&](Head& h) {
+      h.sc = scales_of(p.by_tiles.quotient(h.x), h.chunk_id * p.chunk + kUnitKeys * lane, h.entry);
+    };
     int issued = 0;                       // stages sent so far, over all items
     bool ok = true;
+    Head head;
+    head.x = blockIdx.x; head.b = blockIdx.y; head.chunk_id = blockIdx.z;
+    fetch(head);
+    first_scales(head);
     for (int n_item = 0; ok; ++n_item) {
-      bool asked = false;
-      const int hk = x / p.tiles, tile = x - hk * p.tiles, row0 = tile * kRowsTile;
-      const int len = length_of(p, b);
-      const int n_vis = visible(p, len, (min(row0 + kRowsTile, p.rows) - 1) / p.group);
-      const int c_begin = min(chunk_id * p.chunk, n_vis);
+      bool asked = false, known = !p.take_over, more = false, scaled = !p.take_over;   // of the next item
+      Head next;
+      const int hk = p.by_tiles.quotient(head.x), row0 = p.by_tiles.remainder(head.x) * kRowsTile;
+      const int len = min(max(head.len, 0), p.max_len);
+      const int n_vis = visible(p, len, p.by_group.quotient(min(row0 + kRowsTile, p.rows) - 1));
+      const int c_begin = min(head.chunk_id * p.chunk, n_vis);
       const int c_end = min(n_vis, c_begin + p.chunk);
       const int n_stages = (c_end - c_begin + kStageKeys - 1) / kStageKeys;
-      // Lane i looks after unit i of the next four stages: its page, asked for a batch ahead, and
-      // its scales, asked for half a batch ahead.
-      const int32_t* pages = p.table + (long long)b * p.width;
-      auto page_of = [&](int t) -> int {
-        if (t >= c_end) return -1;
-        const int e = pages[t / p.page_size];
-        return e >= 0 && e < p.num_pages ? e : -1;
-      };
-      auto scales_of = [&](int t, int page) -> float2 {
-        if (page < 0) return make_float2(0.f, 0.f);
-        const int blk = t % p.page_size / p.block;
-        return make_float2(p.ks[page * p.ks_sp + blk * p.ks_sb + hk * p.ks_sh],
-                           p.vs[page * p.vs_sp + blk * p.vs_sb + hk * p.vs_sh]);
-      };
-      int t_mine = c_begin + kUnitKeys * lane;
-      int page = page_of(t_mine), page_nx = page_of(t_mine + 32 * kUnitKeys);
-      float2 sc = scales_of(t_mine, page), sc_nx = make_float2(0.f, 0.f);
-      // the item's query rows, and what they are divided by so that fp16 holds them
-      constexpr int kVec = DP / 8;        // 16-byte pieces of a row
-      uint4 qv[kRowsTile * kVec / 32];
-#pragma unroll
-      for (int i = 0; i < kRowsTile * kVec / 32; ++i) {
-        const int r = row0 + (lane + 32 * i) / kVec, c = (lane + 32 * i) % kVec;
-        qv[i] = make_uint4(0, 0, 0, 0);
-        if (r < p.rows && 8 * c < p.head_dim)
-          qv[i] = *reinterpret_cast<const uint4*>((const T*)p.q + b * p.q_sb + r / p.group * p.q_st +
-                                                  (hk * p.group + r % p.group) * p.q_sh + 8 * c);
-      }
+      const int ask_at = max(n_stages - 8, 0), fetch_at = max(n_stages - 5, 1), scales_at = max(n_stages - 2, 2);
+      // lane i looks after unit i of four stages
+      const int32_t* pages = p.table + (long long)head.b * p.width;
+      int t_mine = head.chunk_id * p.chunk + kUnitKeys * lane;
+      int entry = head.entry, entry_nx = head.entry_nx, entry_nx2 = -1, page = -1, row_mine = 0;
+      float2 sc = make_float2(0.f, 0.f), sc_nx = head.sc;
       auto publish = [&]() -> bool {
         if (!warp_wait(item_empty, (n_item & 1) ^ 1)) return false;
+        // (bf16 rows are divided by a power of two so that fp16 holds them)
 #pragma unroll
-        for (int i = 0; i < kRowsTile * kVec / 32; ++i) {
+        for (int i = 0; i < kQRows * kVec / 32; ++i) {
           const int r = (lane + 32 * i) / kVec, c = (lane + 32 * i) % kVec;
-          uint4 v = qv[i];
+          uint4 v = head.q[i];
           float up = 1.f;
           if (std::is_same<T, __nv_bfloat16>::value) {
             unsigned top = __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu),
@@ -262,71 +305,104 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
           if (c == 0) row_scale[r] = up;
         }
         if (lane == 0) {
-          item->x = x; item->b = b; item->chunk_id = chunk_id;
+          item->x = head.x; item->b = head.b; item->chunk_id = head.chunk_id;
           item->c_begin = c_begin; item->c_end = c_end; item->len = len; item->valid = 1;
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(item_full);
         return true;
       };
-      // The first item's copies leave before its query rows have arrived; later ones find the ring
-      // full of the item before.
-      const int publish_at = n_item == 0 ? min(n_stages, L::kStages) - 1 : -1;
+      // the item that comes after this one, and its loads
+      auto look_ahead = [&]() -> bool {
+        if (!warp_wait(next_full, n_item & 1)) return false;
+        known = true;
+        more = next_cta(sbase + L::kNext, next.x, next.b, next.chunk_id);
+        __syncwarp();
+        fence_proxy_async();     // the answer has been read: the next request may overwrite it
+        if (more) fetch(next);
+        else scaled = true;
+        return true;
+      };
+      // The first item's copies leave before its query rows have arrived; later items have the
+      // consumers at work on the one before.
+      const int publish_at = n_item == 0 ? min(n_stages, L::kStages) - 1 : min(n_stages, 1) - 1;
       if (publish_at < 0) ok = publish();
       for (int st = 0; ok && st < max(n_stages, 1); ++st) {
-        if (p.take_over && st == max(n_stages - 2, 0) && lane == 0) {   // what comes after this item
+        if (p.take_over && st == ask_at && lane == 0) {                 // what comes after this item
           mbar_expect_tx(next_full, 16);
           try_cancel_next_cta(sbase + L::kNext, next_full);
           asked = true;
         }
         if (n_stages == 0) break;
-        if (st > 0 && (st & 3) == 0) {                                  // the next batch of units
-          t_mine += 32 * kUnitKeys;
-          page = page_nx; sc = sc_nx;
-          page_nx = page_of(t_mine + 32 * kUnitKeys);
+        if ((st & 3) == 0) {                                            // the next batch of units
+          if (st > 0) { t_mine += kBatch; entry = entry_nx; entry_nx = entry_nx2; }
+          sc = sc_nx;
+          page = t_mine < c_end && entry >= 0 && entry < p.num_pages ? entry : -1;
+          row_mine = p.by_page.remainder(t_mine);
+          entry_nx2 = -1;
+          if (t_mine + 2 * kBatch < c_end) entry_nx2 = pages[p.by_page.quotient(t_mine + 2 * kBatch)];
+          sc_nx = make_float2(0.f, 0.f);
+          if (t_mine + kBatch < c_end) sc_nx = scales_of(hk, t_mine + kBatch, entry_nx);
         }
-        if ((st & 3) == 2) sc_nx = scales_of(t_mine + 32 * kUnitKeys, page_nx);
         const int s = issued % L::kStages;
-        const int v0 = c_begin + st * kStageKeys;
         const int unit0 = kUnits * (st & 3);                            // the stage's first unit = its lane
-        if (!warp_wait(empty(s), ((issued / L::kStages) & 1) ^ 1)) { ok = false; break; }
         const unsigned there = __ballot_sync(0xffffffffu, page >= 0) >> unit0 & ((1u << kUnits) - 1u);
+        if (!warp_wait(empty(s), ((issued / L::kStages) & 1) ^ 1)) { ok = false; break; }
         if (lane >= unit0 && lane < unit0 + kUnits) {
           unit_scales[s * kUnits + lane - unit0].x = sc.x;
           unit_scales[s * kUnits + lane - unit0].y = sc.y;
         }
-        if (lane == 0) unit_mask[s] = there;
-        // a lane per copy: its box's first unit's lane
-        const int per_box = p.box_keys / kUnitKeys, u = lane - unit0;
-        const bool mine = u >= 0 && u < kUnits && u % per_box == 0 && page >= 0;
-        const unsigned copies = __popc(__ballot_sync(0xffffffffu, mine));
         __syncwarp();                                                   // (the scales before the arrival)
-        if (lane == 0) mbar_expect_tx(full(s), copies * 2 * p.box_keys * DP);
-        __syncwarp();
-        if (mine) {
-          const uint32_t kdst = sbase + s * L::kStageBytes + u * kUnitKeys * DP, vdst = kdst + L::kTileBytes;
-          const int r = (v0 + u * kUnitKeys) % p.page_size;
-          tma_load_4d(kdst, &tmap_k, full(s), 0, r, hk, page);
-          tma_load_4d(vdst, &tmap_v, full(s), 0, r, hk, page);
+        // One lane issues, from registers that hold every box: copies of several lanes go out one by one
+        // all the same, and a shuffle between two copies costs as much as a copy.
+        auto copy_stage = [&](auto units) {
+          constexpr int kPer = decltype(units)::value, kBoxes = kUnits / kPer;
+          int pg[kBoxes], row[kBoxes], n = 0;
+#pragma unroll
+          for (int i = 0; i < kBoxes; ++i) {
+            pg[i] = __shfl_sync(0xffffffffu, page, unit0 + i * kPer);
+            row[i] = __shfl_sync(0xffffffffu, row_mine, unit0 + i * kPer);
+            n += pg[i] >= 0;
+          }
+          if (lane == 0) {
+            unit_mask[s] = there;
+            mbar_expect_tx(full(s), n * 2 * kPer * kUnitKeys * DP);
+            const uint32_t kdst = sbase + s * L::kStageBytes, vdst = kdst + L::kTileBytes;
+#pragma unroll
+            for (int i = 0; i < kBoxes; ++i)
+              if (pg[i] >= 0) {
+                tma_load_4d(kdst + i * kPer * kUnitKeys * DP, &tmap_k, full(s), 0, row[i], hk, pg[i]);
+                tma_load_4d(vdst + i * kPer * kUnitKeys * DP, &tmap_v, full(s), 0, row[i], hk, pg[i]);
+              }
+          }
+        };
+        switch (p.box_keys) {
+          case 16: copy_stage(std::integral_constant<int, 1>()); break;
+          case 32: copy_stage(std::integral_constant<int, 2>()); break;
+          case 64: copy_stage(std::integral_constant<int, 4>()); break;
+          default: copy_stage(std::integral_constant<int, 8>()); break;
         }
         __syncwarp();
         ++issued;
         if (st == publish_at) ok = publish();
+        if (ok && !known && st >= fetch_at) ok = look_ahead();
+        else if (known && !scaled && st >= scales_at) { first_scales(next); scaled = true; }
       }
+      if (ok && !known) ok = look_ahead();
+      if (ok && !scaled) first_scales(next);
       // (the answer writes shared memory, so it is waited for whatever happened)
       asked = __shfl_sync(0xffffffffu, asked ? 1 : 0, 0) != 0;
-      if (!ok || (p.take_over && !warp_wait(next_full, n_item & 1))) {
+      if (!ok) {
         if (asked) mbar_drain(next_full, n_item & 1);
         break;
       }
-      if (!p.take_over || !next_cta(sbase + L::kNext, x, b, chunk_id)) {
+      if (!more) {
         if (warp_wait(item_empty, n_item & 1)) {
           if (lane == 0) { item->valid = 0; mbar_arrive(item_full); }
         }
         break;
       }
-      __syncwarp();
-      fence_proxy_async();     // the answer has been read: the next request may overwrite it
+      head = next;
     }
     // A wait gave up somewhere in the CTA: the consumers no longer wait for the stages, so
     // the copies still in flight are waited for here before the CTA may exit.
@@ -337,9 +413,8 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
 
   // ================================================================== consumers
   const int gid = lane >> 2, tig = lane & 3;
-  float* sm_fold = reinterpret_cast<float*>(sgen + L::kFold);
-  float* sm_m = reinterpret_cast<float*>(sgen + L::kMl);               // [4][16]
-  float* sm_l = sm_m + 4 * 16;
+  float* sm_m = reinterpret_cast<float*>(sgen + L::kMl);               // [warps][16]
+  float* sm_l = sm_m + kConsumers * 16;
   // the 16-byte piece `c` of row `r` of a tile (64- or 128-byte swizzle of the copy engine)
   auto piece = [](int r, int c) -> uint32_t {
     return r * DP + ((DP == 128 ? c ^ (r & 7) : c ^ ((r >> 1) & 3)) << 4);
@@ -354,9 +429,9 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
     const int x = item->x, b = item->b, chunk_id = item->chunk_id;
     const int c_begin = item->c_begin, c_end = item->c_end, len = item->len;
     const int n_stages = (c_end - c_begin + kStageKeys - 1) / kStageKeys;
-    const int hk = x / p.tiles, row0 = (x - hk * p.tiles) * kRowsTile;
+    const int hk = p.by_tiles.quotient(x), row0 = p.by_tiles.remainder(x) * kRowsTile;
     const int rows_here = min(kRowsTile, p.rows - row0);
-    const int query0 = row0 / p.group, query1 = (row0 + rows_here - 1) / p.group;
+    const int query0 = p.by_group.quotient(row0), query1 = p.by_group.quotient(row0 + rows_here - 1);
     unsigned qa[kQJ][4][2 * kNT];          // A operand of step m of piece j: rows gid (and gid + 8)
     float rsc[kNT];                        // what the scores of the lane's rows are multiplied by, but for ks
     int query[kNT], limit[kNT];            // the query of the row, the keys it sees
@@ -370,7 +445,7 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
         qa[j][2][r] = c.x; qa[j][2][kNT + r] = c.y; qa[j][3][r] = c.z; qa[j][3][kNT + r] = c.w;
       }
       rsc[r] = row_scale[gid + 8 * r] * p.scale_log2;
-      query[r] = min(row0 + gid + 8 * r, p.rows - 1) / p.group;
+      query[r] = p.by_group.quotient(min(row0 + gid + 8 * r, p.rows - 1));
       limit[r] = min(visible(p, len, query[r]), c_end);
     }
     const int limit0 = min(visible(p, len, query0), c_end);   // keys that every row of the tile sees
@@ -535,11 +610,11 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
         }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(empty(s));
+      if (lane == 0 && st + 1 < n_stages) mbar_arrive(empty(s));
     }
 
-    // ---- fold the four warps' sums, 32 or 64 columns at a time, through a buffer beside the ring
-    constexpr int kCols = kRows == 8 ? 64 : 32, kPitch = kCols + 4;
+    // ---- fold the warps' sums in the buffer of the item's last stage, which is given back only then
+    // (the producer is filling the others for the next item)
 #pragma unroll
     for (int r = 0; r < kNT; ++r) {
       l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 1);
@@ -549,53 +624,63 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
         sm_l[warp * 16 + gid + 8 * r] = l_run[r];
       }
     }
-    bool gave_up = false;
+    const int last = (used + L::kStages - 1) % L::kStages;
+    float* sm_fold = reinterpret_cast<float*>(sgen + last * L::kStageBytes);   // [warps][rows][DP]
+    // (a bounded wait gave up: the chunk is reported as empty and the caller is told through the status word)
+    const bool gave_up = consumers_any(*abort_flag != 0);        // (and everyone has read the stage)
+    const bool sums = n_stages > 0 && !gave_up;
+    if (sums) {
+      // the columns of rows 2 tig and 2 tig + 1 are moved by 8 tig, so that a store's four row pairs
+      // lie in banks of their own
 #pragma unroll
-    for (int rd = 0; rd < DP / kCols; ++rd) {
-#pragma unroll
-      for (int i = 0; i < kCols / 16; ++i)
+      for (int c = 0; c < kChunks16; ++c)
 #pragma unroll
         for (int r = 0; r < kNT; ++r) {
-          const float* a4 = acc[(kCols / 16) * rd + i][r];
-          float* at = sm_fold + (warp * kRows + 8 * r + 2 * tig) * kPitch + 16 * i + 2 * gid;
-          *reinterpret_cast<float2*>(at) = make_float2(a4[0], a4[2]);
-          *reinterpret_cast<float2*>(at + kPitch) = make_float2(a4[1], a4[3]);
+          float* at = sm_fold + (warp * kRows + 8 * r + 2 * tig) * DP + ((16 * c + 2 * gid) ^ (8 * tig));
+          *reinterpret_cast<float2*>(at) = make_float2(acc[c][r][0], acc[c][r][2]);
+          *reinterpret_cast<float2*>(at + DP) = make_float2(acc[c][r][1], acc[c][r][3]);
         }
-      // (a bounded wait gave up: the chunk is reported as empty and the caller is told through the
-      // status word)
-      gave_up = consumers_any(*abort_flag != 0) || gave_up;
-      for (int g = warp; g < rows_here; g += 4) {
-        float M = -INFINITY;
+    }
+    asm volatile("bar.sync 1, %0;" ::"n"(32 * kConsumers) : "memory");
+    // a thread takes four columns of a row
+    constexpr int kLanes = DP / 4;
+    for (int i = threadIdx.x; i < rows_here * kLanes; i += 32 * kConsumers) {
+      const int g = i / kLanes, d = 4 * (i % kLanes);
+      float M = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) M = fmaxf(M, sm_m[w * 16 + g]);
-        const float Ms = (M == -INFINITY) ? 0.f : M;
-        float f[4], Lsum = 0.f;
+      for (int w = 0; w < kConsumers; ++w) M = fmaxf(M, sm_m[w * 16 + g]);
+      const float Ms = (M == -INFINITY) ? 0.f : M;
+      float Lsum = 0.f;
+      float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          f[w] = exp2f(sm_m[w * 16 + g] - Ms);
-          Lsum += sm_l[w * 16 + g] * f[w];
+      for (int w = 0; w < kConsumers; ++w) {
+        const float f = exp2f(sm_m[w * 16 + g] - Ms);
+        Lsum += sm_l[w * 16 + g] * f;
+        if (sums) {
+          const float4 v = *reinterpret_cast<const float4*>(sm_fold + (w * kRows + g) * DP + (d ^ (8 * ((g & 7) >> 1))));
+          O.x += v.x * f; O.y += v.y * f; O.z += v.z * f; O.w += v.w * f;
         }
-        const bool some = Lsum != 0.f && !gave_up;
-        const int row = row0 + g;
-        const long long prow = ((long long)(b * p.heads_kv + hk) * p.rows + row) * p.max_chunks + chunk_id;
-        T* orow = (T*)p.o + b * p.o_sb + row / p.group * p.o_st + (hk * p.group + row % p.group) * p.o_sh;
-#pragma unroll
-        for (int cc = 0; cc < kCols; cc += 32) {
-          float O = 0.f;
-#pragma unroll
-          for (int w = 0; w < 4; ++w) O += sm_fold[(w * kRows + g) * kPitch + cc + lane] * f[w];
-          const float v = some ? O / Lsum : 0.f;
-          const int d = kCols * rd + cc + lane;
-          if (d < p.head_dim) {
-            if (p.direct_o) orow[d] = from_float<T>(v);
-            else p.part_o[prow * p.head_dim + d] = v;
-          }
-        }
-        if (rd == 0 && lane == 0 && !p.direct_o) p.part_lse[prow] = some ? Ms - kPUp + log2f(Lsum) : -INFINITY;
       }
-      asm volatile("bar.sync 1, 128;" ::: "memory");
+      const bool some = Lsum != 0.f && sums;
+      O = some ? make_float4(O.x / Lsum, O.y / Lsum, O.z / Lsum, O.w / Lsum) : make_float4(0.f, 0.f, 0.f, 0.f);
+      const int row = row0 + g;
+      const long long prow = ((long long)(b * p.heads_kv + hk) * p.rows + row) * p.max_chunks + chunk_id;
+      if (d < p.head_dim) {
+        if (p.direct_o) {
+          T* at = (T*)p.o + b * p.o_sb + p.by_group.quotient(row) * p.o_st +
+                  (hk * p.group + p.by_group.remainder(row)) * p.o_sh + d;
+          at[0] = from_float<T>(O.x); at[1] = from_float<T>(O.y);
+          at[2] = from_float<T>(O.z); at[3] = from_float<T>(O.w);
+        } else {
+          *reinterpret_cast<float4*>(p.part_o + prow * p.head_dim + d) = O;
+        }
+      }
+      if (d == 0 && !p.direct_o) p.part_lse[prow] = some ? Ms - kPUp + log2f(Lsum) : -INFINITY;
     }
     if (gave_up) break;
+    fence_proxy_async();       // the plain accesses to the stage come before the copy engine's next write
+    __syncwarp();
+    if (lane == 0 && n_stages > 0) mbar_arrive(empty(last));
   }
   if (threadIdx.x == 0 && *abort_flag && p.status_word) atomicExch(p.status_word, 1);
 }
@@ -609,8 +694,9 @@ __global__ void __launch_bounds__(32 * kCombineWarps) decode_8bit_combine_kernel
   sm100::grid_dependency_wait();
   constexpr int kLanes = D / 4;                     // lanes that hold 4 columns each
   const int hk = blockIdx.x / p.rows, row = blockIdx.x - hk * p.rows, b = blockIdx.y;
+  const int query = p.by_group.quotient(row), head = p.by_group.remainder(row);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n = visible(p, length_of(p, b), row / p.group);
+  const int n = visible(p, length_of(p, b), query);
   const int nchunk = (n + p.chunk - 1) / p.chunk;
   const long long row0 = ((long long)(b * p.heads_kv + hk) * p.rows + row) * p.max_chunks;
   const float* lse = p.part_lse + row0;
@@ -643,7 +729,7 @@ __global__ void __launch_bounds__(32 * kCombineWarps) decode_8bit_combine_kernel
     float s = 0.f;
 #pragma unroll
     for (int w = 0; w < kCombineWarps; ++w) s += reinterpret_cast<const float*>(part[w])[d];
-    T* orow = (T*)p.o + b * p.o_sb + row / p.group * p.o_st + (hk * p.group + row % p.group) * p.o_sh;
+    T* orow = (T*)p.o + b * p.o_sb + query * p.o_st + (hk * p.group + head) * p.o_sh;
     orow[d] = from_float<T>(s);
   }
 }
@@ -744,7 +830,7 @@ int launch_split(const b200attn_paged_decode_8bit_args* a, const Decode8Params& 
   if (!pool_map(&tk, a->k_pages, a, a->k_stride_t, a->k_stride_h, a->k_stride_page, DP, p.box_keys) ||
       !pool_map(&tv, a->v_pages, a, a->v_stride_t, a->v_stride_h, a->v_stride_page, DP, p.box_keys))
     return B200ATTN_ERR_CUDA;
-  return launch_after(kernel, grid, dim3(160), L::kAlloc, stream, tk, tv, p) == cudaSuccess ? B200ATTN_OK
+  return launch_after(kernel, grid, dim3(kDecode8Threads), L::kAlloc, stream, tk, tv, p) == cudaSuccess ? B200ATTN_OK
                                                                                             : B200ATTN_ERR_CUDA;
 }
 template <typename T, bool kE4M3>
@@ -797,7 +883,9 @@ int paged_decode_8bit_fwd(const b200attn_paged_decode_8bit_args* a, cudaStream_t
   p.batch = a->batch; p.queries = a->queries; p.heads_kv = a->heads_kv;
   p.group = a->heads_q / a->heads_kv; p.head_dim = a->head_dim;
   p.rows = (int)rows; p.tiles = (int)tiles;
-  p.page_size = a->page_size; p.block = a->block_tokens; p.num_pages = a->num_pages; p.width = a->max_pages_per_seq;
+  p.by_page = divisor(a->page_size); p.by_group = divisor(p.group); p.by_tiles = divisor((int)tiles);
+  p.block_shift = a->block_tokens == 16 ? 4 : a->block_tokens == 32 ? 5 : a->block_tokens == 64 ? 6 : 7;
+  p.num_pages = a->num_pages; p.width = a->max_pages_per_seq;
   p.max_len = (int)max_visible(a);
   p.box_keys = std::min(a->page_size & -a->page_size, kStageKeys);
   p.chunk = chunk_of(a); p.max_chunks = (int)chunks;
