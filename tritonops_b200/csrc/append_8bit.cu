@@ -26,6 +26,7 @@ namespace {
 
 constexpr int kAppendThreads = 256;
 constexpr int kAppendWarps = kAppendThreads / 32;
+constexpr int kCtasPerSm = 2;
 constexpr int kMaxBlockTokens = 128;
 constexpr int kUnitRows = 16;
 
@@ -104,34 +105,105 @@ __device__ __forceinline__ float4 unquantise4(unsigned q) {
                      (float)(signed char)(q >> 24));
 }
 
+// What a block's numbers are divided by and turned into, given the maximum over its new rows and the
+// scale `before` of its earlier ones (0: none).
 template <typename T, bool kE4M3>
-__global__ void __launch_bounds__(kAppendThreads) append_8bit_kernel(const AppendParams p) {
+struct Scaling {
+  float before, after, inv;
+  bool pow2, stored;
+  __device__ __forceinline__ Scaling(unsigned top, float before_) : before(before_) {
+    const float need = scale_for<T, kE4M3>(top);
+    after = (need != need || before != before) ? __uint_as_float(0x7fc00000u) : fmaxf(need, before);
+    // the reciprocal of a power of two is exact; scales that came from elsewhere are divided by
+    const unsigned bits = __float_as_uint(after);
+    pow2 = (bits & 0x7fffffu) == 0 && bits >= 0x00800000u && bits < 0x7f000000u;
+    inv = pow2 ? __uint_as_float(0x7f000000u - bits) : 0.f;
+    stored = after > 0.f;                      // (false for NaN: numbers of such a block are 0)
+  }
+  __device__ __forceinline__ float over(float v) const { return !stored ? 0.f : pow2 ? v * inv : __fdiv_rn(v, after); }
+  __device__ __forceinline__ unsigned four(unsigned lo, unsigned hi) const {
+    const float2 a = unpack2<T>(lo), b = unpack2<T>(hi);
+    return quantise4<kE4M3>(over(a.x), over(a.y), over(b.x), over(b.y));
+  }
+  __device__ __forceinline__ uint2 eight(const uint4& x) const { return make_uint2(four(x.x, x.y), four(x.z, x.w)); }
+  // eight numbers of an earlier row to the new scale
+  __device__ __forceinline__ uint2 again(const uint2& old) const {
+    const float ratio = __fdiv_rn(before, after);
+    const float4 a = unquantise4<kE4M3>(old.x), c = unquantise4<kE4M3>(old.y);
+    return make_uint2(quantise4<kE4M3>(a.x * ratio, a.y * ratio, a.z * ratio, a.w * ratio),
+                      quantise4<kE4M3>(c.x * ratio, c.y * ratio, c.z * ratio, c.w * ratio));
+  }
+};
+__device__ __forceinline__ unsigned max_abs_of(const uint4& x) {
+  const unsigned m = max_abs16(max_abs16(max_abs16(x.x & 0x7fff7fffu, x.y), x.z), x.w);
+  return max(m & 0xffffu, m >> 16);
+}
+
+// One new row for each sequence: a few kilobytes, so the time is the chain of look-ups (length, page,
+// scale).  A group of head_dim / 8 lanes takes the row of one (sequence, head, K or V), which it asks
+// for before it knows where it goes, and nothing is shared between groups.
+template <typename T, bool kE4M3>
+__global__ void __launch_bounds__(kAppendThreads) append_8bit_one_kernel(const AppendParams p) {
+  sm100::launch_dependents();
+  const int lane = threadIdx.x & 31, lanes = p.head_dim >> 3, at_once = 32 / lanes;
+  const int mine = lane / lanes, col = (lane - mine * lanes) * 8;
+  const int job = (blockIdx.x * kAppendWarps + (threadIdx.x >> 5)) * at_once + mine;
+  const bool some = mine < at_once && job < 2 * p.tokens * p.heads;
+  const int which = job & 1, t = (job >> 1) / p.heads, h = (job >> 1) % p.heads;
+  sm100::grid_dependency_wait();
+  if (!some) return;
+  const uint4 x = *reinterpret_cast<const uint4*>((const T*)p.rows[which] + (long long)t * p.row_st[which] +
+                                                  h * p.row_sh[which] + col);
+  const int len = p.lens[t];
+  if (len < 0 || len / p.page_size >= p.width) return;
+  const int page = p.table[(long long)t * p.width + len / p.page_size];
+  if (page < 0 || page >= p.num_pages) return;
+  const int in_page = len % p.page_size, index = in_page / p.block, off = in_page % p.block;
+  float* scale = p.scales[which] + page * p.scale_sp[which] + index * p.scale_sb[which] + h * p.scale_sh[which];
+  unsigned char* base = (unsigned char*)p.pages[which] + page * p.page_sp[which] +
+                        (long long)index * p.block * p.page_st[which] + h * p.page_sh[which] + col;
+  const unsigned group = (lanes == 32 ? 0xffffffffu : (1u << lanes) - 1u) << (mine * lanes);
+  const float before = off ? *scale : 0.f;
+  const unsigned top = __reduce_max_sync(group, max_abs_of(x));
+  const Scaling<T, kE4M3> sc(top, before);
+  *reinterpret_cast<uint2*>(base + off * p.page_st[which]) = sc.eight(x);
+  if (off && sc.after > before) {              // (eight rows' loads together: the others wait for this)
+    for (int r0 = 0; r0 < off; r0 += 8) {
+      uint2 old[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (r0 + i < off) old[i] = *reinterpret_cast<const uint2*>(base + (r0 + i) * p.page_st[which]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (r0 + i < off) *reinterpret_cast<uint2*>(base + (r0 + i) * p.page_st[which]) = sc.again(old[i]);
+    }
+  }
+  __syncwarp(group);                           // (the others have read the scale)
+  if (col == 0) *scale = sc.after;
+}
+
+// Packed new rows.  The loads of the next task are under way while a warp works on one.
+template <typename T, bool kE4M3>
+__global__ void __launch_bounds__(kAppendThreads, 2) append_8bit_kernel(const AppendParams p) {
   __shared__ AppendBlock blocks[kMaxBlockTokens];
   __shared__ int n_blocks;
-  __shared__ unsigned tops[kAppendWarps];
+  __shared__ unsigned tops[2][kAppendWarps];
   sm100::launch_dependents();
   if (threadIdx.x == 0) n_blocks = 0;
   sm100::grid_dependency_wait();
   // ---- which blocks begin to be written in this tile
   const int t0 = blockIdx.x * p.tile;
-  int b = t0;
-  if (p.cu) {
-    b = 0;                                     // sequences that end at or before t0
-    for (int i0 = 0; i0 < p.batch; i0 += kAppendThreads) {
-      const int i = i0 + threadIdx.x;
-      b += __syncthreads_count(i < p.batch && p.cu[i + 1] <= t0);
-    }
+  int b = 0;                                   // sequences that end at or before t0
+  for (int i0 = 0; i0 < p.batch; i0 += kAppendThreads) {
+    const int i = i0 + threadIdx.x;
+    b += __syncthreads_count(i < p.batch && p.cu[i + 1] <= t0);
   }
   __syncthreads();
   const int t = t0 + threadIdx.x;
   if ((int)threadIdx.x < p.tile && t < p.tokens) {
     int first = t, end = t + 1;
-    if (p.cu) {
-      while (b < p.batch && p.cu[b + 1] <= t) ++b;
-      if (b < p.batch) { first = p.cu[b]; end = min(p.cu[b + 1], p.tokens); }
-    } else {
-      b = t;
-    }
+    while (b < p.batch && p.cu[b + 1] <= t) ++b;
+    if (b < p.batch) { first = p.cu[b]; end = min(p.cu[b + 1], p.tokens); }
     if (b < p.batch && first >= 0 && first <= t) {
       const int len = p.lens[b];
       const long long pos = (long long)len + (t - first);
@@ -149,95 +221,81 @@ __global__ void __launch_bounds__(kAppendThreads) append_8bit_kernel(const Appen
   __syncthreads();
   // ---- the tasks
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int groups = kAppendWarps / p.warps_per_task, group = warp / p.warps_per_task;
-  const int w = warp - group * p.warps_per_task;
+  const int wpt = p.warps_per_task, groups = kAppendWarps / wpt, group = warp / wpt, w = warp - group * wpt;
   const int job0 = blockIdx.y * p.jobs_per_cta, n_jobs = min(p.jobs_per_cta, 2 * p.heads - job0);
   const int n_tasks = n_blocks * n_jobs;
   const int lanes = p.head_dim >> 3, rows_at_once = 32 / lanes;      // a lane holds 8 numbers of a row
   const int my_row = lane / lanes, my_col = (lane - my_row * lanes) * 8;
   const bool active = my_row < rows_at_once;
-  for (int task0 = 0; task0 < n_tasks; task0 += groups) {
-    const int task = task0 + group;
-    const bool some = task < n_tasks;
-    AppendBlock g = {};
-    int which = 0, h = 0;
-    uint4 x[kUnitRows / 2];
-    unsigned top = 0;
-    float before = 0.f;
-    float* scale = nullptr;
-    unsigned char* base = nullptr;
-    int unit = 0;                              // the warp's unit with new rows
-    if (some) {
-      g = blocks[task / n_jobs];
-      const int job = job0 + task % n_jobs;
-      which = job & 1; h = job >> 1;
-      scale = p.scales[which] + g.page * p.scale_sp[which] + g.index * p.scale_sb[which] + h * p.scale_sh[which];
-      base = (unsigned char*)p.pages[which] + g.page * p.page_sp[which] +
-             (long long)g.index * p.block * p.page_st[which] + h * p.page_sh[which];
-      if (g.off) before = *scale;
-      unit = p.warps_per_task == 1 ? g.off / kUnitRows : w;
-      const T* rows = (const T*)p.rows[which] + h * p.row_sh[which] + my_col;
-#pragma unroll
-      for (int i = 0; i < kUnitRows / 2; ++i) {
-        const int r = unit * kUnitRows + i * rows_at_once + my_row - g.off;      // of the block's new rows
-        x[i] = make_uint4(0, 0, 0, 0);
-        if (active && i * rows_at_once < kUnitRows && r >= 0 && r < g.fresh)
-          x[i] = *reinterpret_cast<const uint4*>(rows + (long long)(g.row0 + r) * p.row_st[which]);
-      }
-#pragma unroll
-      for (int i = 0; i < kUnitRows / 2; ++i)
-        top = max_abs16(max_abs16(max_abs16(max_abs16(top, x[i].x), x[i].y), x[i].z), x[i].w);
-      top = max(top & 0xffffu, top >> 16);
-      top = __reduce_max_sync(0xffffffffu, top);
-    }
-    if (p.warps_per_task > 1) {
-      __syncthreads();                         // (the task before has read them)
-      if (lane == 0) tops[warp] = top;
-      __syncthreads();
-      for (int i = 0; i < p.warps_per_task; ++i) top = max(top, tops[group * p.warps_per_task + i]);
-    }
-    if (!some) continue;
-    const float need = scale_for<T, kE4M3>(top);
-    const float after = (need != need || before != before) ? __uint_as_float(0x7fc00000u) : fmaxf(need, before);
-    // the reciprocal of a power of two is exact; scales that came from elsewhere are divided by
-    const unsigned bits = __float_as_uint(after);
-    const bool pow2 = (bits & 0x7fffffu) == 0 && bits >= 0x00800000u && bits < 0x7f000000u;
-    const float inv = pow2 ? __uint_as_float(0x7f000000u - bits) : 0.f;
-    const bool stored = after > 0.f;           // (false for NaN: numbers of such a block are 0)
-    auto over = [&](float v) { return !stored ? 0.f : pow2 ? v * inv : __fdiv_rn(v, after); };
+  struct Task {
+    uint4 x[kUnitRows / 2];                    // the warp's rows of the block
+    float before;
+    int row0, off, fresh, which;
+    float* scale;
+    unsigned char* base;
+  };
+  auto load = [&](int task, Task& k) {
+    if (task >= n_tasks) return;
+    const AppendBlock g = blocks[task / n_jobs];
+    const int job = job0 + task % n_jobs, h = job >> 1;
+    k.which = job & 1; k.off = g.off; k.fresh = g.fresh;
+    k.scale = p.scales[k.which] + g.page * p.scale_sp[k.which] + g.index * p.scale_sb[k.which] + h * p.scale_sh[k.which];
+    k.base = (unsigned char*)p.pages[k.which] + g.page * p.page_sp[k.which] +
+             (long long)g.index * p.block * p.page_st[k.which] + h * p.page_sh[k.which];
+    k.before = 0.f;
+    if (g.off) k.before = *k.scale;
+    const T* rows = (const T*)p.rows[k.which] + h * p.row_sh[k.which] + my_col;
 #pragma unroll
     for (int i = 0; i < kUnitRows / 2; ++i) {
-      const int r = unit * kUnitRows + i * rows_at_once + my_row;                // of the block
-      if (active && i * rows_at_once < kUnitRows && r >= g.off && r - g.off < g.fresh) {
-        const float2 a = unpack2<T>(x[i].x), c = unpack2<T>(x[i].y), d = unpack2<T>(x[i].z), e = unpack2<T>(x[i].w);
-        const uint2 q = make_uint2(quantise4<kE4M3>(over(a.x), over(a.y), over(c.x), over(c.y)),
-                                   quantise4<kE4M3>(over(d.x), over(d.y), over(e.x), over(e.y)));
-        *reinterpret_cast<uint2*>(base + r * p.page_st[which] + my_col) = q;
+      const int r = w * kUnitRows + i * rows_at_once + my_row - g.off;           // of the block's new rows
+      k.x[i] = make_uint4(0, 0, 0, 0);
+      if (active && i * rows_at_once < kUnitRows && r >= 0 && r < g.fresh)
+        k.x[i] = *reinterpret_cast<const uint4*>(rows + (long long)(g.row0 + r) * p.row_st[k.which]);
+    }
+  };
+  Task now, next;
+  load(group, now);
+  for (int task0 = 0, turn = 0; task0 < n_tasks; task0 += groups, turn ^= 1) {
+    const bool some = task0 + group < n_tasks;
+    load(task0 + groups + group, next);
+    unsigned top = 0;
+    if (some) {
+#pragma unroll
+      for (int i = 0; i < kUnitRows / 2; ++i) top = max(top, max_abs_of(now.x[i]));
+      top = __reduce_max_sync(0xffffffffu, top);
+    }
+    if (wpt > 1) {                             // the warps of a task meet (two sets of places, one barrier)
+      if (lane == 0) tops[turn][warp] = top;
+      __syncthreads();
+      for (int i = 0; i < wpt; ++i) top = max(top, tops[turn][group * wpt + i]);
+    }
+    if (some) {
+      const Scaling<T, kE4M3> sc(top, now.before);
+      unsigned char* const base = now.base + my_col;
+      const long long st = p.page_st[now.which];
+#pragma unroll
+      for (int i = 0; i < kUnitRows / 2; ++i) {
+        const int r = w * kUnitRows + i * rows_at_once + my_row;                 // of the block
+        if (active && i * rows_at_once < kUnitRows && r >= now.off && r - now.off < now.fresh)
+          *reinterpret_cast<uint2*>(base + r * st) = sc.eight(now.x[i]);
+        else if (active && i * rows_at_once < kUnitRows && r < now.off && sc.after > now.before)
+          *reinterpret_cast<uint2*>(base + r * st) = sc.again(*reinterpret_cast<const uint2*>(base + r * st));
       }
+      if (w == 0 && lane == 0) *now.scale = sc.after;
     }
-    if (g.off && after > before) {             // earlier rows of the block to the new scale
-      const float ratio = __fdiv_rn(before, after);
-      for (int u = w; u * kUnitRows < g.off; u += p.warps_per_task)
-        for (int i = 0; i * rows_at_once < kUnitRows; ++i) {
-          const int r = u * kUnitRows + i * rows_at_once + my_row;
-          if (active && r < g.off) {
-            uint2* at = reinterpret_cast<uint2*>(base + r * p.page_st[which] + my_col);
-            const uint2 old = *at;
-            const float4 a = unquantise4<kE4M3>(old.x), c = unquantise4<kE4M3>(old.y);
-            *at = make_uint2(quantise4<kE4M3>(a.x * ratio, a.y * ratio, a.z * ratio, a.w * ratio),
-                             quantise4<kE4M3>(c.x * ratio, c.y * ratio, c.z * ratio, c.w * ratio));
-          }
-        }
-    }
-    if (w == 0 && lane == 0) *scale = after;
+    now = next;
   }
 }
 
-template <typename T>
-cudaError_t launch_append(const b200attn_kv_append_8bit_args* a, const AppendParams& p, dim3 grid, cudaStream_t stream) {
-  return a->cache_dtype == B200ATTN_E4M3
-             ? launch_after(append_8bit_kernel<T, true>, grid, dim3(kAppendThreads), 0, stream, p)
-             : launch_after(append_8bit_kernel<T, false>, grid, dim3(kAppendThreads), 0, stream, p);
+template <typename T, bool kE4M3>
+cudaError_t launch_append(const AppendParams& p, cudaStream_t stream) {
+  if (!p.cu) {
+    const int jobs = 2 * p.tokens * p.heads, each = kAppendWarps * (32 / (p.head_dim / 8));
+    return launch_after(append_8bit_one_kernel<T, kE4M3>, dim3((jobs + each - 1) / each), dim3(kAppendThreads), 0, stream, p);
+  }
+  const dim3 grid((unsigned)((p.tokens + p.tile - 1) / p.tile),
+                  (unsigned)((2 * p.heads + p.jobs_per_cta - 1) / p.jobs_per_cta));
+  return launch_after(append_8bit_kernel<T, kE4M3>, grid, dim3(kAppendThreads), 0, stream, p);
 }
 
 }  // namespace
@@ -257,6 +315,7 @@ int kv_append_8bit(const b200attn_kv_append_8bit_args* a, cudaStream_t stream) {
     return B200ATTN_ERR_MODE;
   if (a->page_size <= 0 || a->page_size % a->block_tokens != 0) return B200ATTN_ERR_MODE;
   if (a->tokens > INT_MAX - kMaxBlockTokens || a->heads > 16384) return B200ATTN_ERR_TOO_LARGE;
+  if (!a->cu_new && 2 * a->tokens * a->heads > INT_MAX - 65536) return B200ATTN_ERR_TOO_LARGE;
   const void* ptrs[4] = {a->new_k, a->new_v, a->k_pages, a->v_pages};
   for (const void* q : ptrs)
     if ((uintptr_t)q & 15) return B200ATTN_ERR_ALIGN;
@@ -268,7 +327,8 @@ int kv_append_8bit(const b200attn_kv_append_8bit_args* a, cudaStream_t stream) {
                               a->v_stride_page, a->v_stride_t, a->v_stride_h};
   for (long long s : pools)
     if (s % 16 != 0) return B200ATTN_ERR_STRIDE;
-  if (int st = device_info(nullptr)) return st;
+  const DeviceInfo* di = nullptr;
+  if (int st = device_info(&di)) return st;
   set_launch_count(0);
   if (a->tokens == 0) return B200ATTN_OK;
   AppendParams p;
@@ -284,15 +344,17 @@ int kv_append_8bit(const b200attn_kv_append_8bit_args* a, cudaStream_t stream) {
   p.table = a->page_table; p.lens = a->seqlens; p.cu = a->cu_new;
   p.tokens = (int)a->tokens; p.batch = a->batch; p.heads = a->heads; p.head_dim = a->head_dim;
   p.page_size = a->page_size; p.block = a->block_tokens; p.num_pages = a->num_pages; p.width = a->max_pages_per_seq;
-  // One new token each: a CTA per token and eight (head, K or V) pairs, a warp each.  Packed rows: a
-  // CTA looks after a block's worth of them, with a warp for each of a block's units.
-  p.tile = a->cu_new ? a->block_tokens : 1;
-  p.warps_per_task = a->cu_new ? a->block_tokens / kUnitRows : 1;
-  p.jobs_per_cta = std::min(kAppendWarps / p.warps_per_task, 2 * a->heads);
-  const dim3 grid((unsigned)((a->tokens + p.tile - 1) / p.tile),
-                  (unsigned)((2 * a->heads + p.jobs_per_cta - 1) / p.jobs_per_cta));
-  const cudaError_t e = a->dtype == B200ATTN_F16 ? launch_append<__half>(a, p, grid, stream)
-                                                 : launch_append<__nv_bfloat16>(a, p, grid, stream);
+  // Packed rows: a CTA looks after a block's worth of them, with a warp for each of a block's units, and
+  // after all heads where that still fills the chip twice over.
+  p.tile = a->block_tokens;
+  p.warps_per_task = a->block_tokens / kUnitRows;
+  const int tiles = (int)((a->tokens + p.tile - 1) / p.tile), at_once = kAppendWarps / p.warps_per_task;
+  const int splits = std::max(1, std::min((2 * kCtasPerSm * di->sm_count + tiles - 1) / tiles, (2 * a->heads + at_once - 1) / at_once));
+  p.jobs_per_cta = ((2 * a->heads + splits - 1) / splits + at_once - 1) / at_once * at_once;
+  const bool e4m3 = a->cache_dtype == B200ATTN_E4M3;
+  const cudaError_t e = a->dtype == B200ATTN_F16 ? (e4m3 ? launch_append<__half, true>(p, stream) : launch_append<__half, false>(p, stream))
+                                                 : (e4m3 ? launch_append<__nv_bfloat16, true>(p, stream)
+                                                         : launch_append<__nv_bfloat16, false>(p, stream));
   if (e != cudaSuccess) return B200ATTN_ERR_CUDA;
   set_launch_count(1);
   return cudaGetLastError() == cudaSuccess ? B200ATTN_OK : B200ATTN_ERR_CUDA;

@@ -21,6 +21,7 @@ namespace {
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWarps = kPlanThreads / 32;
 constexpr int kPlanCtas = 8;             // the largest portable cluster
+constexpr long long kOneCta = 8192;      // entries and pages that one CTA goes through alone
 constexpr int kMaxSlots = 32768;         // slots of a fork: their keepers stay in shared memory
 constexpr int kHeader = 64;              // ints at the front of every workspace
 constexpr int kCopies = 0, kCountA = 8, kCountB = 24, kCountC = 40;   // in the header: copies, counts per CTA
@@ -41,17 +42,12 @@ __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 
-// Sum of `v` before this thread in the CTA; `total` is the CTA's.  Ends with a barrier.
-__device__ __forceinline__ int block_before(int v, int& total) {
+// Of a value that a warp's lanes share, the sum over the warps before this one; `total` is the CTA's.
+// Ends with a barrier.
+__device__ __forceinline__ int warps_before(int v, int& total) {
   __shared__ int sums[kPlanWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int incl = v;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int t = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += t;
-  }
-  if (lane == 31) sums[warp] = incl;
+  if (lane == 0) sums[warp] = v;
   __syncthreads();
   int s = sums[lane];
 #pragma unroll
@@ -62,32 +58,56 @@ __device__ __forceinline__ int block_before(int v, int& total) {
   const int base = __shfl_sync(0xffffffffu, s, (warp + 31) & 31);
   total = __shfl_sync(0xffffffffu, s, 31);
   __syncthreads();
-  return incl - v + (warp ? base : 0);
+  return warp ? base : 0;
 }
 __device__ __forceinline__ int block_sum(int v) {
   int total;
-  block_before(v, total);
+  warps_before(__reduce_add_sync(0xffffffffu, v), total);
   return total;
 }
 
-// emit(i, rank) for the i in [lo, hi) with pred(i), ascending, ranks from `rank0`, those below `limit`.
-template <typename Pred, typename Emit>
-__device__ __forceinline__ void enumerate(int lo, int hi, int rank0, int limit, Pred pred, Emit emit) {
-  constexpr int kPer = 4;
-  for (int start = lo; start < hi && rank0 < limit; start += kPer * kPlanThreads) {
-    const int i0 = start + kPer * threadIdx.x;
-    unsigned mask = 0;
+// f(i, value(i)) for the i in [lo, hi), kAhead loads of a thread in flight together: a CTA has one
+// thousand threads for lists of up to hundreds of thousands, so a load at a time would cost its latency
+// hundreds of times over (1024 rows of 537 entries and 327,000 pages: 62 us a hand-out).
+constexpr int kAhead = 8;
+template <typename Value, typename F>
+__device__ __forceinline__ void each(int lo, int hi, int step, Value value, F f) {
+  for (long long i0 = lo; i0 < hi; i0 += (long long)kAhead * step) {
+    int v[kAhead];
 #pragma unroll
-    for (int j = 0; j < kPer; ++j)
-      if (i0 + j < hi && pred(i0 + j)) mask |= 1u << j;
-    int total;
-    int rank = rank0 + block_before(__popc(mask), total);
+    for (int j = 0; j < kAhead; ++j)
+      if (i0 + j * step < hi) v[j] = value((int)(i0 + j * step));
 #pragma unroll
-    for (int j = 0; j < kPer; ++j)
-      if ((mask >> j) & 1u) {
-        if (rank < limit) emit(i0 + j, rank);
-        ++rank;
-      }
+    for (int j = 0; j < kAhead; ++j)
+      if (i0 + j * step < hi) f((int)(i0 + j * step), v[j]);
+  }
+}
+
+// emit(i, rank) for the i in [lo, hi) with pred(value(i)), ascending, ranks from `rank0`, those below
+// `limit`.  A warp takes 256 neighbours at a time.
+template <typename Value, typename Pred, typename Emit>
+__device__ __forceinline__ void enumerate(int lo, int hi, int rank0, int limit, Value value, Pred pred, Emit emit) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (long long start = lo; start < hi && rank0 < limit; start += kAhead * kPlanThreads) {
+    const long long i0 = start + warp * (32 * kAhead) + lane;
+    int v[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (i0 + 32 * j < hi) v[j] = value((int)(i0 + 32 * j));
+    unsigned has[kAhead];
+    int count = 0, total;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      has[j] = __ballot_sync(0xffffffffu, i0 + 32 * j < hi && pred(v[j]));
+      count += __popc(has[j]);
+    }
+    int rank = rank0 + warps_before(count, total);
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int mine = rank + __popc(has[j] & ((1u << lane) - 1u));
+      if (((has[j] >> lane) & 1u) && mine < limit) emit((int)(i0 + 32 * j), mine);
+      rank += __popc(has[j]);
+    }
     rank0 += total;
   }
 }
@@ -120,7 +140,9 @@ struct GrowParams {
   int32_t* missing;
   int slots, width, pages, page_size;
   int* header;
-  int* need;       // [slots] pages a row lacks, then the pages that the rows before it lack
+  int* need;       // [slots] pages a row lacks
+  int* first;      // [slots] the first entry that does
+  int* rank0;      // [slots] pages that the rows before lack
   int* free_list;  // [pages]
 };
 
@@ -137,22 +159,20 @@ __global__ void __launch_bounds__(kPlanThreads, 1) grow_kernel(const GrowParams 
   int lo, hi;
   segment(p.pages, lo, hi);
   int free_here = 0;
-  for (int i = lo + threadIdx.x; i < hi; i += kPlanThreads) {
-    const int r = p.refs[i];
-    p.refs_out[i] = r;
-    free_here += r <= 0;
-  }
+  each(lo + threadIdx.x, hi, kPlanThreads, [&](int i) { return p.refs[i]; },
+       [&](int i, int r) { p.refs_out[i] = r; free_here += r <= 0; });
   for (int b = warp; b < p.slots; b += warps) {
+    const long long row = (long long)b * p.width;
     const int want = (int)min((long long)p.width, pages_wanted(p, b));
-    int lacks = 0;
-    for (int i = lane; i < p.width; i += 32) {
-      const int e = p.table[(long long)b * p.width + i];
+    int lacks = 0, first = INT_MAX;      // entries without a page, the first of them
+    each(lane, p.width, 32, [&](int i) { return p.table[row + i]; }, [&](int i, int e) {
       const bool held = e >= 0 && e < p.pages;
-      p.table_out[(long long)b * p.width + i] = held ? e : -1;
-      lacks += i < want && !held;
-    }
+      p.table_out[row + i] = held ? e : -1;
+      if (i < want && !held) { ++lacks; first = min(first, i); }
+    });
     lacks = __reduce_add_sync(0xffffffffu, lacks);
-    if (lane == 0) p.need[b] = lacks;
+    first = __reduce_min_sync(0xffffffffu, first);
+    if (lane == 0) { p.need[b] = lacks; p.first[b] = first; }
   }
   free_here = block_sum(free_here);
   if (threadIdx.x == 0) p.header[kCountA + cluster_rank()] = free_here;
@@ -160,36 +180,40 @@ __global__ void __launch_bounds__(kPlanThreads, 1) grow_kernel(const GrowParams 
 
   int free_before, free_all, asked = 0;
   counts_of(p.header + kCountA, free_before, free_all);
-  for (int b = threadIdx.x; b < p.slots; b += kPlanThreads) asked += __ldcg(p.need + b);
+  each(threadIdx.x, p.slots, kPlanThreads, [&](int b) { return __ldcg(p.need + b); }, [&](int, int n) { asked += n; });
   asked = block_sum(asked);
-  enumerate(lo, hi, free_before, asked, [&](int i) { return p.refs[i] <= 0; },
+  enumerate(lo, hi, free_before, asked, [&](int i) { return p.refs[i]; }, [](int r) { return r <= 0; },
             [&](int i, int rank) { p.free_list[rank] = i; });
-  cluster_barrier();      // (everyone has read `need` as it was)
-  if (cluster_rank() == 0) {
+  if (cluster_rank() == cluster_size() - 1) {          // what the rows before each lack
     long long over = 0;
     for (int b = threadIdx.x; b < p.slots; b += kPlanThreads) over += max(pages_wanted(p, b) - p.width, 0LL);
     __shared__ unsigned long long over_all;
     if (threadIdx.x == 0) over_all = 0;
     __syncthreads();
     if (over) atomicAdd(&over_all, (unsigned long long)over);
-    int run = 0;
-    for (int start = 0; start < p.slots; start += kPlanThreads) {
+    for (int start = 0, run = 0; start < p.slots; start += kPlanThreads) {
       const int b = start + threadIdx.x;
-      int total;
-      const int before = block_before(b < p.slots ? __ldcg(p.need + b) : 0, total);
-      if (b < p.slots) p.need[b] = run + before;
+      int n = b < p.slots ? __ldcg(p.need + b) : 0, total;
+      const int own = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int t = __shfl_up_sync(0xffffffffu, n, o);
+        if (lane >= o) n += t;
+      }
+      const int before = run + warps_before(__shfl_sync(0xffffffffu, n, 31), total) + n - own;
+      if (b < p.slots) p.rank0[b] = before;
       run += total;
     }
-    __syncthreads();
     if (threadIdx.x == 0)
       *p.missing = (int)min((long long)INT_MAX, (long long)over_all + max(asked - free_all, 0));
   }
   cluster_barrier();
 
   for (int b = warp; b < p.slots; b += warps) {
+    if (__ldcg(p.need + b) == 0) continue;
     const int want = (int)min((long long)p.width, pages_wanted(p, b));
-    int rank = __ldcg(p.need + b);
-    for (int i0 = 0; i0 < want; i0 += 32) {
+    int rank = __ldcg(p.rank0 + b);
+    for (int i0 = __ldcg(p.first + b); i0 < want; i0 += 32) {
       const int i = i0 + lane;
       int32_t* entry = p.table_out + (long long)b * p.width + i;
       const bool lacks = i < want && __ldcg(entry) < 0;
@@ -235,7 +259,7 @@ __global__ void __launch_bounds__(kPlanThreads, 1) fork_kernel(const ForkParams 
     const int parent = p.parents[b];
     if (parent >= 0 && parent < p.slots) atomicMin(&keeper[parent], parent == b ? -1 : b);
   }
-  for (int i = tid; i < p.pages; i += threads) p.refs_out[i] = p.refs[i];
+  each(tid, p.pages, threads, [&](int i) { return p.refs[i]; }, [&](int i, int r) { p.refs_out[i] = r; });
   cluster_barrier();
 
   for (int b = warp; b < p.slots; b += warps) {
@@ -246,18 +270,18 @@ __global__ void __launch_bounds__(kPlanThreads, 1) fork_kernel(const ForkParams 
     const int full = len / p.page_size;
     const bool part = len % p.page_size != 0;
     int copy = -1;
-    for (int i = lane; i < p.width; i += 32) {
-      int e = alive ? p.table[(long long)parent * p.width + i] : -1;
+    const int32_t* theirs = p.table + (long long)parent * p.width;
+    const long long row = (long long)b * p.width;
+    each(lane, p.width, 32, [&](int i) { return alive ? theirs[i] : -1; }, [&](int i, int e) {
       if (e >= p.pages) e = -1;
       const int taken = e >= 0 && (keeps || i < full) ? e : -1;
-      if (!stays) {
-        const int old = p.table[(long long)b * p.width + i];
-        if (old >= 0 && old < p.pages) atomicSub(p.refs_out + old, 1);
-        if (taken >= 0) atomicAdd(p.refs_out + taken, 1);
-      }
-      p.table_out[(long long)b * p.width + i] = taken;
+      if (!stays && taken >= 0) atomicAdd(p.refs_out + taken, 1);
+      p.table_out[row + i] = taken;
       if (part && i == full && !keeps) copy = e;
-    }
+    });
+    if (!stays)
+      each(lane, p.width, 32, [&](int i) { return p.table[row + i]; },
+           [&](int, int old) { if (old >= 0 && old < p.pages) atomicSub(p.refs_out + old, 1); });
     copy = __reduce_max_sync(0xffffffffu, copy);
     if (lane == 0) {
       p.want[b] = copy;
@@ -268,21 +292,22 @@ __global__ void __launch_bounds__(kPlanThreads, 1) fork_kernel(const ForkParams 
 
   int lo, hi, asked = 0, free_here = 0;
   segment(p.pages, lo, hi);
-  for (int b = threadIdx.x; b < p.slots; b += kPlanThreads) asked += __ldcg(p.want + b) >= 0;
+  each(threadIdx.x, p.slots, kPlanThreads, [&](int b) { return __ldcg(p.want + b); }, [&](int, int e) { asked += e >= 0; });
   asked = block_sum(asked);
   if (asked > 0)      // (the same in every CTA)
-    for (int i = lo + threadIdx.x; i < hi; i += kPlanThreads) free_here += __ldcg(p.refs_out + i) <= 0;
+    each(lo + threadIdx.x, hi, kPlanThreads, [&](int i) { return __ldcg(p.refs_out + i); },
+         [&](int, int r) { free_here += r <= 0; });
   free_here = block_sum(free_here);
   if (threadIdx.x == 0) p.header[kCountA + cluster_rank()] = free_here;
   cluster_barrier();
   int free_before, free_all;
   counts_of(p.header + kCountA, free_before, free_all);
-  enumerate(lo, hi, free_before, asked, [&](int i) { return __ldcg(p.refs_out + i) <= 0; },
+  enumerate(lo, hi, free_before, asked, [&](int i) { return __ldcg(p.refs_out + i); }, [](int r) { return r <= 0; },
             [&](int i, int rank) { p.free_list[rank] = i; });
   cluster_barrier();
 
   if (cluster_rank() != 0) return;
-  enumerate(0, p.slots, 0, asked, [&](int b) { return __ldcg(p.want + b) >= 0; }, [&](int b, int rank) {
+  enumerate(0, p.slots, 0, asked, [&](int b) { return __ldcg(p.want + b); }, [](int e) { return e >= 0; }, [&](int b, int rank) {
     const int len = __ldcg(p.lens_out + b), full = len / p.page_size;
     if (rank < free_all) {
       const int page = __ldcg(p.free_list + rank);
@@ -320,18 +345,17 @@ __global__ void __launch_bounds__(kPlanThreads, 1) compact_kernel(const CompactP
   const int tid = cluster_rank() * kPlanThreads + threadIdx.x, threads = cluster_size() * kPlanThreads;
   int lo, hi, count = 0, unused, n;
   segment(p.pages, lo, hi);
-  for (int i = lo + threadIdx.x; i < hi; i += kPlanThreads) count += p.refs[i] > 0;
+  each(lo + threadIdx.x, hi, kPlanThreads, [&](int i) { return p.refs[i]; }, [&](int, int r) { count += r > 0; });
   count = block_sum(count);
   if (threadIdx.x == 0) p.header[kCountA + cluster_rank()] = count;
   cluster_barrier();
   counts_of(p.header + kCountA, unused, n);
 
   int holes = 0, movers = 0;
-  for (int i = lo + threadIdx.x; i < hi; i += kPlanThreads) {
-    const bool in_use = p.refs[i] > 0;
-    holes += i < n && !in_use;
-    movers += i >= n && in_use;
-  }
+  each(lo + threadIdx.x, hi, kPlanThreads, [&](int i) { return p.refs[i]; }, [&](int i, int r) {
+    holes += i < n && r <= 0;
+    movers += i >= n && r > 0;
+  });
   holes = block_sum(holes);
   movers = block_sum(movers);
   if (threadIdx.x == 0) {
@@ -342,24 +366,22 @@ __global__ void __launch_bounds__(kPlanThreads, 1) compact_kernel(const CompactP
   int holes_before, movers_before, moves;
   counts_of(p.header + kCountB, holes_before, unused);
   counts_of(p.header + kCountC, movers_before, moves);
-  enumerate(lo, min(hi, n), holes_before, INT_MAX, [&](int i) { return p.refs[i] <= 0; },
+  const auto refs = [&](int i) { return p.refs[i]; };
+  enumerate(lo, min(hi, n), holes_before, INT_MAX, refs, [](int r) { return r <= 0; },
             [&](int i, int rank) { p.dst[rank] = i; p.rank_of[i] = rank; });
-  enumerate(max(lo, n), hi, movers_before, INT_MAX, [&](int i) { return p.refs[i] > 0; },
+  enumerate(max(lo, n), hi, movers_before, INT_MAX, refs, [](int r) { return r > 0; },
             [&](int i, int rank) { p.src[rank] = i; p.rank_of[i] = rank; });
   cluster_barrier();
 
-  for (int i = tid; i < p.pages; i += threads) {
-    int r = i < n ? p.refs[i] : 0;
-    if (i < n && r <= 0) r = p.refs[__ldcg(p.src + __ldcg(p.rank_of + i))];
+  each(tid, p.pages, threads, refs, [&](int i, int r) {
+    if (i >= n) r = 0;
+    else if (r <= 0) r = p.refs[__ldcg(p.src + __ldcg(p.rank_of + i))];
     p.refs_out[i] = r;
-  }
-  const long long entries = (long long)p.slots * p.width;
-  for (long long i = tid; i < entries; i += threads) {
-    int e = p.table[i];
-    if (e < 0 || e >= p.pages || p.refs[e] <= 0) e = -1;
-    else if (e >= n) e = __ldcg(p.dst + __ldcg(p.rank_of + e));
-    p.table_out[i] = e;
-  }
+  });
+  each(tid, p.slots * p.width, threads, [&](int i) {
+    const int e = p.table[i];
+    return e >= 0 && e < p.pages && p.refs[e] > 0 ? e : -1;
+  }, [&](int i, int e) { p.table_out[i] = e < n ? e : __ldcg(p.dst + __ldcg(p.rank_of + e)); });
   if (tid == 0) {
     p.header[kCopies] = moves;
     *p.live = n;
@@ -457,12 +479,13 @@ int check_pools(const b200attn_page_pool* pools, int n) {
 }
 
 template <typename P>
-int launch_plan(void (*kernel)(P), const P& p, size_t smem, cudaStream_t stream) {
+int launch_plan(void (*kernel)(P), const P& p, long long entries, size_t smem, cudaStream_t stream) {
   if (smem > 48 * 1024 &&
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
     return B200ATTN_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(kPlanCtas);
+  const int ctas = entries <= kOneCta ? 1 : kPlanCtas;
+  cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(kPlanThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -470,7 +493,7 @@ int launch_plan(void (*kernel)(P), const P& p, size_t smem, cudaStream_t stream)
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = kPlanCtas;
+  attr[1].val.clusterDim.x = ctas;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
@@ -502,7 +525,7 @@ int launch_copies(const b200attn_page_pool* pools, int n_pools, const int* count
 
 size_t pages_grow_workspace_bytes(const b200attn_pages_grow_args* a) {
   if (!a || a->slots <= 0 || a->num_pages <= 0) return 0;
-  return 4 * ((size_t)kHeader + a->slots + a->num_pages);
+  return 4 * ((size_t)kHeader + 3 * (size_t)a->slots + a->num_pages);
 }
 
 int pages_grow(const b200attn_pages_grow_args* a, cudaStream_t stream) {
@@ -520,8 +543,10 @@ int pages_grow(const b200attn_pages_grow_args* a, cudaStream_t stream) {
   p.slots = a->slots; p.width = a->max_pages_per_seq; p.pages = a->num_pages; p.page_size = a->page_size;
   p.header = (int*)a->workspace;
   p.need = p.header + kHeader;
-  p.free_list = p.need + a->slots;
-  st = launch_plan(grow_kernel, p, 0, stream);
+  p.first = p.need + a->slots;
+  p.rank0 = p.first + a->slots;
+  p.free_list = p.rank0 + a->slots;
+  st = launch_plan(grow_kernel, p, (long long)p.slots * p.width + p.pages, 0, stream);
   if (st != B200ATTN_OK) return st;
   set_launch_count(1);
   return cudaGetLastError() == cudaSuccess ? B200ATTN_OK : B200ATTN_ERR_CUDA;
@@ -557,7 +582,7 @@ int pages_fork(const b200attn_pages_fork_args* a, cudaStream_t stream) {
   p.free_list = p.want + a->slots;
   p.src = p.free_list + a->slots;
   p.dst = p.src + a->slots;
-  st = launch_plan(fork_kernel, p, n, stream);
+  st = launch_plan(fork_kernel, p, (long long)p.slots * p.width + p.pages, n, stream);
   if (st != B200ATTN_OK) return st;
   int launches = 1;
   st = launch_copies(a->pools, a->n_pools, p.header + kCopies, p.src, p.dst, di->sm_count, stream, launches);
@@ -590,7 +615,7 @@ int pages_compact(const b200attn_pages_compact_args* a, cudaStream_t stream) {
   p.rank_of = p.header + kHeader;
   p.src = p.rank_of + a->num_pages;
   p.dst = p.src + a->num_pages;
-  st = launch_plan(compact_kernel, p, 0, stream);
+  st = launch_plan(compact_kernel, p, (long long)p.slots * p.width + p.pages, 0, stream);
   if (st != B200ATTN_OK) return st;
   int launches = 1;
   st = launch_copies(a->pools, a->n_pools, p.header + kCopies, p.src, p.dst, di->sm_count, stream, launches);
