@@ -17,6 +17,7 @@
 #include <limits.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "sm100.cuh"
@@ -80,17 +81,18 @@ __device__ __forceinline__ float scale_for(unsigned top) {
   return __uint_as_float((unsigned)max(s, 1) << 23);    // (not below 2^-126)
 }
 
-// round(x / s), four numbers
+// round(x * inv), four numbers of at most the type's largest.  int8: added to 1.5 * 2^23 a number is rounded
+// to an integer, ties to even, whose low byte it then ends with.
 template <bool kE4M3>
-__device__ __forceinline__ unsigned quantise4(float a, float b, float c, float d) {
+__device__ __forceinline__ unsigned quantise4(float a, float b, float c, float d, float inv) {
   if (kE4M3) {
     unsigned short lo, hi;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b * inv), "f"(a * inv));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d * inv), "f"(c * inv));
     return (unsigned)lo | ((unsigned)hi << 16);
   }
-  auto one = [](float x) { return (unsigned)min(max(__float2int_rn(x), -127), 127) & 255u; };
-  return one(a) | (one(b) << 8) | (one(c) << 16) | (one(d) << 24);
+  auto one = [&](float x) { return __float_as_uint(fmaf(x, inv, 12582912.f)); };
+  return __byte_perm(__byte_perm(one(a), one(b), 0x0040), __byte_perm(one(c), one(d), 0x0040), 0x5410);
 }
 template <bool kE4M3>
 __device__ __forceinline__ float4 unquantise4(unsigned q) {
@@ -110,7 +112,7 @@ __device__ __forceinline__ float4 unquantise4(unsigned q) {
 template <typename T, bool kE4M3>
 struct Scaling {
   float before, after, inv;
-  bool pow2, stored;
+  bool pow2;
   __device__ __forceinline__ Scaling(unsigned top, float before_) : before(before_) {
     const float need = scale_for<T, kE4M3>(top);
     after = (need != need || before != before) ? __uint_as_float(0x7fc00000u) : fmaxf(need, before);
@@ -118,20 +120,31 @@ struct Scaling {
     const unsigned bits = __float_as_uint(after);
     pow2 = (bits & 0x7fffffu) == 0 && bits >= 0x00800000u && bits < 0x7f000000u;
     inv = pow2 ? __uint_as_float(0x7f000000u - bits) : 0.f;
-    stored = after > 0.f;                      // (false for NaN: numbers of such a block are 0)
   }
-  __device__ __forceinline__ float over(float v) const { return !stored ? 0.f : pow2 ? v * inv : __fdiv_rn(v, after); }
-  __device__ __forceinline__ unsigned four(unsigned lo, unsigned hi) const {
-    const float2 a = unpack2<T>(lo), b = unpack2<T>(hi);
-    return quantise4<kE4M3>(over(a.x), over(a.y), over(b.x), over(b.y));
+  // eight numbers of a new row; kPow2: as `pow2` says
+  template <bool kPow2>
+  __device__ __forceinline__ uint2 eight(const uint4& x) const {
+    const unsigned w[4] = {x.x, x.y, x.z, x.w};
+    unsigned q[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float2 a = unpack2<T>(w[2 * i]), b = unpack2<T>(w[2 * i + 1]);
+      if (!kPow2) {
+        auto over = [&](float v) { return after > 0.f ? __fdiv_rn(v, after) : 0.f; };   // (numbers of a NaN block are 0)
+        a = make_float2(over(a.x), over(a.y));
+        b = make_float2(over(b.x), over(b.y));
+      }
+      q[i] = quantise4<kE4M3>(a.x, a.y, b.x, b.y, kPow2 ? inv : 1.f);
+    }
+    return make_uint2(q[0], q[1]);
   }
-  __device__ __forceinline__ uint2 eight(const uint4& x) const { return make_uint2(four(x.x, x.y), four(x.z, x.w)); }
   // eight numbers of an earlier row to the new scale
   __device__ __forceinline__ uint2 again(const uint2& old) const {
     const float ratio = __fdiv_rn(before, after);
     const float4 a = unquantise4<kE4M3>(old.x), c = unquantise4<kE4M3>(old.y);
-    return make_uint2(quantise4<kE4M3>(a.x * ratio, a.y * ratio, a.z * ratio, a.w * ratio),
-                      quantise4<kE4M3>(c.x * ratio, c.y * ratio, c.z * ratio, c.w * ratio));
+    auto times = [&](float v) { return __fmul_rn(v, ratio); };      // (rounded before the number is)
+    return make_uint2(quantise4<kE4M3>(times(a.x), times(a.y), times(a.z), times(a.w), 1.f),
+                      quantise4<kE4M3>(times(c.x), times(c.y), times(c.z), times(c.w), 1.f));
   }
 };
 __device__ __forceinline__ unsigned max_abs_of(const uint4& x) {
@@ -166,7 +179,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_8bit_one_kernel(const A
   const float before = off ? *scale : 0.f;
   const unsigned top = __reduce_max_sync(group, max_abs_of(x));
   const Scaling<T, kE4M3> sc(top, before);
-  *reinterpret_cast<uint2*>(base + off * p.page_st[which]) = sc.eight(x);
+  *reinterpret_cast<uint2*>(base + off * p.page_st[which]) = sc.pow2 ? sc.template eight<true>(x) : sc.template eight<false>(x);
   if (off && sc.after > before) {              // (eight rows' loads together: the others wait for this)
     for (int r0 = 0; r0 < off; r0 += 8) {
       uint2 old[8];
@@ -271,16 +284,25 @@ __global__ void __launch_bounds__(kAppendThreads, 2) append_8bit_kernel(const Ap
     }
     if (some) {
       const Scaling<T, kE4M3> sc(top, now.before);
-      unsigned char* const base = now.base + my_col;
       const long long st = p.page_st[now.which];
+      unsigned char* const base = now.base + my_col + (w * kUnitRows + my_row) * st;
+      const int r0 = w * kUnitRows + my_row - now.off;                           // the lane's first row among the new ones
+      auto store = [&](auto pow2) {
 #pragma unroll
-      for (int i = 0; i < kUnitRows / 2; ++i) {
-        const int r = w * kUnitRows + i * rows_at_once + my_row;                 // of the block
-        if (active && i * rows_at_once < kUnitRows && r >= now.off && r - now.off < now.fresh)
-          *reinterpret_cast<uint2*>(base + r * st) = sc.eight(now.x[i]);
-        else if (active && i * rows_at_once < kUnitRows && r < now.off && sc.after > now.before)
-          *reinterpret_cast<uint2*>(base + r * st) = sc.again(*reinterpret_cast<const uint2*>(base + r * st));
-      }
+        for (int i = 0; i < kUnitRows / 2; ++i) {
+          const int r = r0 + i * rows_at_once;
+          if (active && i * rows_at_once < kUnitRows && r >= 0 && r < now.fresh)
+            *reinterpret_cast<uint2*>(base + i * rows_at_once * st) = sc.template eight<decltype(pow2)::value>(now.x[i]);
+        }
+      };
+      if (sc.pow2) store(std::true_type());
+      else store(std::false_type());
+      if (now.off && sc.after > now.before)                                      // earlier rows to the new scale
+        for (int i = 0; i * rows_at_once < kUnitRows; ++i)
+          if (active && r0 + i * rows_at_once < 0) {
+            uint2* at = reinterpret_cast<uint2*>(base + i * rows_at_once * st);
+            *at = sc.again(*at);
+          }
       if (w == 0 && lane == 0) *now.scale = sc.after;
     }
     now = next;

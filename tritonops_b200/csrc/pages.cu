@@ -39,7 +39,8 @@ __device__ __forceinline__ int cluster_size() {
 // Barrier of all threads of the cluster; what they wrote before it is visible behind it (read with
 // __ldcg where it was written by another CTA of this launch).
 __device__ __forceinline__ void cluster_barrier() {
-  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+  if (cluster_size() == 1) __syncthreads();
+  else asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 
 // Of a value that a warp's lanes share, the sum over the warps before this one; `total` is the CTA's.
@@ -209,22 +210,29 @@ __global__ void __launch_bounds__(kPlanThreads, 1) grow_kernel(const GrowParams 
   }
   cluster_barrier();
 
-  for (int b = warp; b < p.slots; b += warps) {
-    if (__ldcg(p.need + b) == 0) continue;
-    const int want = (int)min((long long)p.width, pages_wanted(p, b));
-    int rank = __ldcg(p.rank0 + b);
-    for (int i0 = __ldcg(p.first + b); i0 < want; i0 += 32) {
-      const int i = i0 + lane;
-      int32_t* entry = p.table_out + (long long)b * p.width + i;
-      const bool lacks = i < want && __ldcg(entry) < 0;
-      const unsigned all = __ballot_sync(0xffffffffu, lacks);
-      const int mine = rank + __popc(all & ((1u << lane) - 1u));
-      if (lacks && mine < free_all) {
-        const int page = __ldcg(p.free_list + mine);
-        *entry = page;
-        p.refs_out[page] = 1;
+  // (a lane looks up one of the warp's rows each; most rows lack their last entries, which then need not
+  // be read again)
+  for (int b0 = warp; b0 < p.slots; b0 += 32 * warps) {
+    const long long looked = min((long long)b0 + (long long)lane * warps, (long long)p.slots - 1);
+    const int all_need = __ldcg(p.need + looked), all_first = __ldcg(p.first + looked), all_rank = __ldcg(p.rank0 + looked);
+    const int all_want = (int)min((long long)p.width, pages_wanted(p, (int)looked));
+    for (int k = 0; k < 32 && b0 + (long long)k * warps < p.slots; ++k) {
+      const int need = __shfl_sync(0xffffffffu, all_need, k), first = __shfl_sync(0xffffffffu, all_first, k),
+                want = __shfl_sync(0xffffffffu, all_want, k);
+      int rank = __shfl_sync(0xffffffffu, all_rank, k);
+      int32_t* row = p.table_out + (b0 + (long long)k * warps) * p.width;
+      for (int i0 = need ? first : want; i0 < want; i0 += 32) {
+        const int i = i0 + lane;
+        const bool lacks = i < want && (need == want - first || __ldcg(row + i) < 0);
+        const unsigned all = __ballot_sync(0xffffffffu, lacks);
+        const int mine = rank + __popc(all & ((1u << lane) - 1u));
+        if (lacks && mine < free_all) {
+          const int page = __ldcg(p.free_list + mine);
+          row[i] = page;
+          p.refs_out[page] = 1;
+        }
+        rank += __popc(all);
       }
-      rank += __popc(all);
     }
   }
 }
