@@ -690,7 +690,8 @@ constexpr int kCombineWarps = 4;
 
 template <typename T, int D>
 __global__ void __launch_bounds__(32 * kCombineWarps) decode_8bit_combine_kernel(const Decode8Params p) {
-  sm100::launch_dependents();
+  // (no kernel may start before this one ends: one that has started keeps what it has read of the partial
+  // sums' memory, which the next call writes again)
   sm100::grid_dependency_wait();
   constexpr int kLanes = D / 4;                     // lanes that hold 4 columns each
   const int hk = blockIdx.x / p.rows, row = blockIdx.x - hk * p.rows, b = blockIdx.y;
@@ -773,16 +774,29 @@ long long rows_of(const b200attn_paged_decode_8bit_args* a) {
   return (long long)a->queries * (a->heads_q / a->heads_kv);
 }
 
-// Split size.
+// Split size: the one with the least waves x (stages of a chunk + 4) + half a chunk + 3 where there is
+// more than one chunk, all lengths taken as the largest.  Four stages are a chunk's own cost (look-ups
+// behind a full ring, the fold), half a chunk the uneven end of a ragged batch, three the second kernel.
+// Measured on B200, 8 KV heads, D = 128, us: 64 sequences of 4096 keys 90.5 in one chunk, 96 in 1024; of
+// 1024-8192 118.7 in 2048, 125 in 1024, 132 in one; 16 of 1024-8192 47.3 in 2048, 44.0 in 1536, 49.6 in
+// 4096; 12 of 4096 26.0 in 1536, 28.6 in 2048; 8 of 2048 13.5 in 512, 15.3 in 768; four of 90001-131072
+// 156.6 in 2048, 151 in 4096, 182 in 8192; one of 8192 10.9 in 256, 13.4 in 128.
+constexpr long long kSlots = 2 * 148;
 int chunk_of(const b200attn_paged_decode_8bit_args* a) {
   if (a->chunk_tokens > 0) return a->chunk_tokens;
   const long long units = a->batch * (long long)a->heads_kv * ((rows_of(a) + kRowsTile - 1) / kRowsTile);
-  const long long keys = std::max<long long>(max_visible(a), 1);
-  if (units >= 256) return 4096;
-  const int sizes[8] = {16384, 8192, 4096, 2048, 1024, 512, 256, 128};
-  for (int c : sizes)
-    if (units * ((keys + c - 1) / c) >= 148) return c;
-  return 128;
+  const long long stages = std::max<long long>((max_visible(a) + kStageKeys - 1) / kStageKeys, 1);
+  long long best = 0, least = 0;
+  auto consider = [&](long long per) {
+    const long long n = (stages + per - 1) / per;
+    const long long cost = 2 * ((units * n + kSlots - 1) / kSlots) * (per + 4) + per + (n > 1 ? 6 : 0);
+    if (!best || cost < least) { best = per; least = cost; }
+  };
+  const int sizes[10] = {1, 2, 3, 4, 6, 8, 12, 16, 32, 64};
+  for (int per : sizes)
+    if (per < stages) consider(per);
+  if (stages <= 64 || !best) consider(stages);
+  return (int)(best * kStageKeys);
 }
 long long chunks_of(const b200attn_paged_decode_8bit_args* a) {
   const long long chunk = chunk_of(a), n = (max_visible(a) + chunk - 1) / chunk;
