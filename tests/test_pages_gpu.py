@@ -251,3 +251,42 @@ def test_refusals():
         ops.compact_pages([pool[:1].expand(20, 16)], table, refs)
     with pytest.raises(RuntimeError, match="CUDA tensors only"):
         ops.compact_pages([pool.cpu()], table, refs)
+
+
+@pytest.mark.parametrize("slots,width,pages,size", [(40, 30, 40000, 16), (300, 90, 60001, 32)])
+def test_books_beyond_shared_memory(slots, width, pages, size):
+    """The form in which a cluster keeps the books and another kernel copies."""
+    from tritonops_b200 import ops
+    table, lens, refs = book(11, slots, width, pages, size, fill=0.6, bad=True)
+    r = random.Random(12)
+    new = torch.tensor([r.randint(0, 5 * size) for _ in range(slots)], dtype=i32)
+    same(ops.grow_pages(table.cuda(), lens.cuda(), refs.cuda(), new.cuda(), page_size=size),
+         orc.grow(table, lens, refs, new, size))
+    pools = [torch.randn(pages, 8), torch.randint(-99, 99, (pages, 12), dtype=torch.int8)]
+    for parents in ([b - b % 4 for b in range(slots)], [r.randrange(-2, slots + 2) for _ in range(slots)]):
+        par = torch.tensor(parents, dtype=i32)
+        dev = [p.cuda() for p in pools]
+        got = ops.fork_pages(dev, table.cuda(), lens.cuda(), refs.cuda(), par.cuda(), page_size=size)
+        want = orc.fork(pools, table, lens, refs, par, size)
+        same(got, want[:4])
+        same(dev, want[4])
+    refs[0], refs[pages // 2] = 2, -3
+    dev = [p.cuda() for p in pools]
+    got = ops.compact_pages(dev, table.cuda(), refs.cuda())
+    want = orc.compact(pools, table, refs)
+    same(got, want[:3])
+    same(dev, want[3])
+
+
+def test_no_page_left():
+    """Pages that cannot be given are counted, forks without one lose what is not in a full page."""
+    from tritonops_b200 import ops
+    table, lens, refs = book(13, 8, 6, 60, 16)
+    refs = torch.where(refs <= 0, 1, refs)          # somebody else holds the rest
+    pool = torch.randn(60, 16)
+    par = torch.tensor([0, 0, 0, 3, 3, 3, 6, 6], dtype=i32)
+    got = ops.fork_pages([pool.cuda()], table.cuda(), lens.cuda(), refs.cuda(), par.cuda(), page_size=16)
+    want = orc.fork([pool], table, lens, refs, par, 16)
+    same(got, want[:4])
+    new = torch.full((8,), 20, dtype=i32)
+    same(ops.grow_pages(table.cuda(), lens.cuda(), refs.cuda(), new.cuda(), page_size=16), orc.grow(table, lens, refs, new, 16))

@@ -471,8 +471,11 @@ PyObject* grow_pages(PyObject*, PyObject* const* x, Py_ssize_t n) {
     at::Tensor out = fresh(table.sizes(), table), refs_out = fresh(refs.sizes(), refs), missing = one_int(refs);
     a.page_table_out = out.data_ptr<int32_t>(); a.page_refs_out = refs_out.data_ptr<int32_t>();
     a.missing_out = missing.data_ptr<int32_t>();
-    at::Tensor ws = scratch(L.pages_grow_workspace_bytes(&a), table);
-    a.workspace = ws.data_ptr(); a.workspace_bytes = (size_t)ws.numel();
+    at::Tensor ws;
+    if (const size_t bytes = L.pages_grow_workspace_bytes(&a)) {
+      ws = scratch(bytes, table);
+      a.workspace = ws.data_ptr(); a.workspace_bytes = (size_t)ws.numel();
+    }
     long long launches;
     const int st = call(L.pages_grow, a, table, launches);
     return answer(st, launches, {out, refs_out, missing});
@@ -494,8 +497,11 @@ PyObject* fork_pages(PyObject*, PyObject* const* x, Py_ssize_t n) {
                lens_out = fresh(lens.sizes(), lens);
     a.page_table_out = out.data_ptr<int32_t>(); a.page_refs_out = refs_out.data_ptr<int32_t>();
     a.seqlens_out = lens_out.data_ptr<int32_t>(); a.missing_out = missing.data_ptr<int32_t>();
-    at::Tensor ws = scratch(L.pages_fork_workspace_bytes(&a), table);
-    a.workspace = ws.data_ptr(); a.workspace_bytes = (size_t)ws.numel();
+    at::Tensor ws;
+    if (const size_t bytes = L.pages_fork_workspace_bytes(&a)) {
+      ws = scratch(bytes, table);
+      a.workspace = ws.data_ptr(); a.workspace_bytes = (size_t)ws.numel();
+    }
     long long launches;
     const int st = call(L.pages_fork, a, table, launches);
     return answer(st, launches, {out, lens_out, refs_out, missing});
@@ -514,8 +520,11 @@ PyObject* compact_pages(PyObject*, PyObject* const* x, Py_ssize_t n) {
     at::Tensor out = fresh(table.sizes(), table), refs_out = fresh(refs.sizes(), refs), live = one_int(refs);
     a.page_table_out = out.data_ptr<int32_t>(); a.page_refs_out = refs_out.data_ptr<int32_t>();
     a.live_out = live.data_ptr<int32_t>();
-    at::Tensor ws = scratch(L.pages_compact_workspace_bytes(&a), table);
-    a.workspace = ws.data_ptr(); a.workspace_bytes = (size_t)ws.numel();
+    at::Tensor ws;
+    if (const size_t bytes = L.pages_compact_workspace_bytes(&a)) {
+      ws = scratch(bytes, table);
+      a.workspace = ws.data_ptr(); a.workspace_bytes = (size_t)ws.numel();
+    }
     long long launches;
     const int st = call(L.pages_compact, a, table, launches);
     return answer(st, launches, {out, refs_out, live});

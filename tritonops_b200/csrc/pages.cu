@@ -4,10 +4,13 @@
 //
 // State: the page table [slots, width] and a count per page of the rows that hold it.  Which pages
 // move where is an ordered enumeration (the i-th free page for the i-th place that needs one), so
-// the results are a pure function of the inputs; the steps of one call depend on one another, so
-// its bookkeeping is one cluster of CTAs with cluster barriers between the steps (a few hundred
-// nanoseconds each, against microseconds for a launch), and the pages themselves are then copied by
-// a second kernel that fills the chip and takes the list from memory: the host fetches nothing.
+// the results are a pure function of the inputs.  The host fetches nothing, and the steps of one call
+// depend on one another, so there are two forms:
+//   * Where a CTA can keep the bookkeeping in shared memory (up to some ten thousand pages), every CTA of
+//     the copying grid works it out for itself from the same inputs, writes its share of the new tables
+//     and copies its share of the pages: one launch, nothing exchanged.
+//   * Beyond, one cluster of CTAs keeps the books (cluster barriers between the steps: a few hundred
+//     nanoseconds, against microseconds for a launch) and a second kernel copies from its list.
 #include <limits.h>
 
 #include <algorithm>
@@ -19,9 +22,7 @@ namespace b200attn {
 namespace {
 
 constexpr int kPlanThreads = 1024;
-constexpr int kPlanWarps = kPlanThreads / 32;
 constexpr int kPlanCtas = 8;             // the largest portable cluster
-constexpr long long kOneCta = 8192;      // entries and pages that one CTA goes through alone
 constexpr int kMaxSlots = 32768;         // slots of a fork: their keepers stay in shared memory
 constexpr int kHeader = 64;              // ints at the front of every workspace
 constexpr int kCopies = 0, kCountA = 8, kCountB = 24, kCountC = 40;   // in the header: copies, counts per CTA
@@ -39,18 +40,17 @@ __device__ __forceinline__ int cluster_size() {
 // Barrier of all threads of the cluster; what they wrote before it is visible behind it (read with
 // __ldcg where it was written by another CTA of this launch).
 __device__ __forceinline__ void cluster_barrier() {
-  if (cluster_size() == 1) __syncthreads();
-  else asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 
 // Of a value that a warp's lanes share, the sum over the warps before this one; `total` is the CTA's.
 // Ends with a barrier.
 __device__ __forceinline__ int warps_before(int v, int& total) {
-  __shared__ int sums[kPlanWarps];
+  __shared__ int sums[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (lane == 0) sums[warp] = v;
   __syncthreads();
-  int s = sums[lane];
+  int s = lane < blockDim.x >> 5 ? sums[lane] : 0;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int t = __shfl_up_sync(0xffffffffu, s, o);
@@ -84,12 +84,30 @@ __device__ __forceinline__ void each(int lo, int hi, int step, Value value, F f)
   }
 }
 
+// f(b, i, value(b, i)) for every entry i < width of the rows b < slots, by `warps` warps of which this is
+// number `warp`: eight rows at a time, so that no entry's row has to be divided for.
+template <typename Value, typename F>
+__device__ __forceinline__ void each_entry(int slots, int width, int warp, int warps, Value value, F f) {
+  const int lane = threadIdx.x & 31;
+  for (long long b0 = (long long)warp * kAhead; b0 < slots; b0 += (long long)warps * kAhead)
+    for (int i = lane; i < width; i += 32) {
+      int v[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j)
+        if (b0 + j < slots) v[j] = value((int)b0 + j, i);
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j)
+        if (b0 + j < slots) f((int)b0 + j, i, v[j]);
+    }
+}
+
 // emit(i, rank) for the i in [lo, hi) with pred(value(i)), ascending, ranks from `rank0`, those below
-// `limit`.  A warp takes 256 neighbours at a time.
+// `limit`; the number of ranks counted, at least `limit` if there are as many.  A warp takes 256 neighbours
+// at a time.
 template <typename Value, typename Pred, typename Emit>
-__device__ __forceinline__ void enumerate(int lo, int hi, int rank0, int limit, Value value, Pred pred, Emit emit) {
+__device__ __forceinline__ int enumerate(int lo, int hi, int rank0, int limit, Value value, Pred pred, Emit emit) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (long long start = lo; start < hi && rank0 < limit; start += kAhead * kPlanThreads) {
+  for (long long start = lo; start < hi && rank0 < limit; start += kAhead * blockDim.x) {
     const long long i0 = start + warp * (32 * kAhead) + lane;
     int v[kAhead];
 #pragma unroll
@@ -111,6 +129,7 @@ __device__ __forceinline__ void enumerate(int lo, int hi, int rank0, int limit, 
     }
     rank0 += total;
   }
+  return rank0;
 }
 
 // this CTA's part of [0, n)
@@ -152,6 +171,68 @@ __device__ __forceinline__ long long pages_wanted(const GrowParams& p, int b) {
   return (tokens + p.page_size - 1) / p.page_size;
 }
 
+// A warp copies row b, its entries without a page as -1, and finds how many of those the coming tokens
+// need, and the first of them.
+__device__ __forceinline__ void look_at_row(const GrowParams& p, int b, int& lacks, int& first) {
+  const long long row = (long long)b * p.width;
+  const int want = (int)min((long long)p.width, pages_wanted(p, b));
+  lacks = 0; first = INT_MAX;
+  each(threadIdx.x & 31, p.width, 32, [&](int i) { return p.table[row + i]; }, [&](int i, int e) {
+    const bool held = e >= 0 && e < p.pages;
+    p.table_out[row + i] = held ? e : -1;
+    if (i < want && !held) { ++lacks; first = min(first, i); }
+  });
+  lacks = __reduce_add_sync(0xffffffffu, lacks);
+  first = __reduce_min_sync(0xffffffffu, first);
+}
+// A warp gives row b the pages free_list[rank ..] for its `need` entries that lack one (`rank` below
+// `free_all` only).  Most rows lack their last entries, which then need not be read again.
+template <typename FreeList>
+__device__ __forceinline__ void give(const GrowParams& p, long long b, int need, int first, int want, int rank, int free_all,
+                                     FreeList free_list) {
+  const int lane = threadIdx.x & 31;
+  int32_t* row = p.table_out + b * p.width;
+  for (int i0 = need ? first : want; i0 < want; i0 += 32) {
+    const int i = i0 + lane;
+    const bool lacks = i < want && (need == want - first || __ldcg(row + i) < 0);
+    const unsigned all = __ballot_sync(0xffffffffu, lacks);
+    const int mine = rank + __popc(all & ((1u << lane) - 1u));
+    if (lacks && mine < free_all) {
+      const int page = free_list(mine);
+      row[i] = page;
+      p.refs_out[page] = 1;
+    }
+    rank += __popc(all);
+  }
+}
+// rank0[b]: what the rows before b lack, by one CTA; `missing` is told.  need(b) may be read by everyone.
+template <typename Need>
+__device__ __forceinline__ void rank_rows(const GrowParams& p, int* rank0, int asked, int free_all, Need need) {
+  const int lane = threadIdx.x & 31;
+  __shared__ unsigned long long over;
+  if (threadIdx.x == 0) over = 0;
+  __syncthreads();
+  for (int start = 0, run = 0; start < p.slots; start += blockDim.x) {
+    const int b = start + threadIdx.x;
+    const int own = b < p.slots ? need(b) : 0;
+    if (b < p.slots) {
+      const long long past = pages_wanted(p, b) - p.width;
+      if (past > 0) atomicAdd(&over, (unsigned long long)past);
+    }
+    int n = own, total;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int t = __shfl_up_sync(0xffffffffu, n, o);
+      if (lane >= o) n += t;
+    }
+    const int before = run + warps_before(__shfl_sync(0xffffffffu, n, 31), total) + n - own;
+    if (b < p.slots) rank0[b] = before;
+    run += total;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) *p.missing = (int)min((long long)INT_MAX, (long long)over + max(asked - free_all, 0));
+}
+
 __global__ void __launch_bounds__(kPlanThreads, 1) grow_kernel(const GrowParams p) {
   sm100::launch_dependents();
   sm100::grid_dependency_wait();
@@ -163,16 +244,8 @@ __global__ void __launch_bounds__(kPlanThreads, 1) grow_kernel(const GrowParams 
   each(lo + threadIdx.x, hi, kPlanThreads, [&](int i) { return p.refs[i]; },
        [&](int i, int r) { p.refs_out[i] = r; free_here += r <= 0; });
   for (int b = warp; b < p.slots; b += warps) {
-    const long long row = (long long)b * p.width;
-    const int want = (int)min((long long)p.width, pages_wanted(p, b));
-    int lacks = 0, first = INT_MAX;      // entries without a page, the first of them
-    each(lane, p.width, 32, [&](int i) { return p.table[row + i]; }, [&](int i, int e) {
-      const bool held = e >= 0 && e < p.pages;
-      p.table_out[row + i] = held ? e : -1;
-      if (i < want && !held) { ++lacks; first = min(first, i); }
-    });
-    lacks = __reduce_add_sync(0xffffffffu, lacks);
-    first = __reduce_min_sync(0xffffffffu, first);
+    int lacks, first;
+    look_at_row(p, b, lacks, first);
     if (lane == 0) { p.need[b] = lacks; p.first[b] = first; }
   }
   free_here = block_sum(free_here);
@@ -181,60 +254,55 @@ __global__ void __launch_bounds__(kPlanThreads, 1) grow_kernel(const GrowParams 
 
   int free_before, free_all, asked = 0;
   counts_of(p.header + kCountA, free_before, free_all);
-  each(threadIdx.x, p.slots, kPlanThreads, [&](int b) { return __ldcg(p.need + b); }, [&](int, int n) { asked += n; });
+  const auto need = [&](int b) { return __ldcg(p.need + b); };
+  each(threadIdx.x, p.slots, kPlanThreads, need, [&](int, int n) { asked += n; });
   asked = block_sum(asked);
   enumerate(lo, hi, free_before, asked, [&](int i) { return p.refs[i]; }, [](int r) { return r <= 0; },
             [&](int i, int rank) { p.free_list[rank] = i; });
-  if (cluster_rank() == cluster_size() - 1) {          // what the rows before each lack
-    long long over = 0;
-    for (int b = threadIdx.x; b < p.slots; b += kPlanThreads) over += max(pages_wanted(p, b) - p.width, 0LL);
-    __shared__ unsigned long long over_all;
-    if (threadIdx.x == 0) over_all = 0;
-    __syncthreads();
-    if (over) atomicAdd(&over_all, (unsigned long long)over);
-    for (int start = 0, run = 0; start < p.slots; start += kPlanThreads) {
-      const int b = start + threadIdx.x;
-      int n = b < p.slots ? __ldcg(p.need + b) : 0, total;
-      const int own = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int t = __shfl_up_sync(0xffffffffu, n, o);
-        if (lane >= o) n += t;
-      }
-      const int before = run + warps_before(__shfl_sync(0xffffffffu, n, 31), total) + n - own;
-      if (b < p.slots) p.rank0[b] = before;
-      run += total;
-    }
-    if (threadIdx.x == 0)
-      *p.missing = (int)min((long long)INT_MAX, (long long)over_all + max(asked - free_all, 0));
-  }
+  if (cluster_rank() == cluster_size() - 1) rank_rows(p, p.rank0, asked, free_all, need);
   cluster_barrier();
 
-  // (a lane looks up one of the warp's rows each; most rows lack their last entries, which then need not
-  // be read again)
-  for (int b0 = warp; b0 < p.slots; b0 += 32 * warps) {
+  for (int b0 = warp; b0 < p.slots; b0 += 32 * warps) {          // a lane looks up one of the warp's rows each
     const long long looked = min((long long)b0 + (long long)lane * warps, (long long)p.slots - 1);
     const int all_need = __ldcg(p.need + looked), all_first = __ldcg(p.first + looked), all_rank = __ldcg(p.rank0 + looked);
     const int all_want = (int)min((long long)p.width, pages_wanted(p, (int)looked));
-    for (int k = 0; k < 32 && b0 + (long long)k * warps < p.slots; ++k) {
-      const int need = __shfl_sync(0xffffffffu, all_need, k), first = __shfl_sync(0xffffffffu, all_first, k),
-                want = __shfl_sync(0xffffffffu, all_want, k);
-      int rank = __shfl_sync(0xffffffffu, all_rank, k);
-      int32_t* row = p.table_out + (b0 + (long long)k * warps) * p.width;
-      for (int i0 = need ? first : want; i0 < want; i0 += 32) {
-        const int i = i0 + lane;
-        const bool lacks = i < want && (need == want - first || __ldcg(row + i) < 0);
-        const unsigned all = __ballot_sync(0xffffffffu, lacks);
-        const int mine = rank + __popc(all & ((1u << lane) - 1u));
-        if (lacks && mine < free_all) {
-          const int page = __ldcg(p.free_list + mine);
-          row[i] = page;
-          p.refs_out[page] = 1;
-        }
-        rank += __popc(all);
-      }
-    }
+    for (int k = 0; k < 32 && b0 + (long long)k * warps < p.slots; ++k)
+      give(p, b0 + (long long)k * warps, __shfl_sync(0xffffffffu, all_need, k), __shfl_sync(0xffffffffu, all_first, k),
+           __shfl_sync(0xffffffffu, all_want, k), __shfl_sync(0xffffffffu, all_rank, k), free_all,
+           [&](int i) { return __ldcg(p.free_list + i); });
   }
+}
+
+// The same by one CTA, with its lists in shared memory: for a small cache what counts is the number of
+// trips to memory one after another.
+constexpr int kGrowOneThreads = 512;
+constexpr long long kGrowOneEntries = 16384, kGrowOneInts = 12288;
+__global__ void __launch_bounds__(kGrowOneThreads, 1) grow_one_kernel(const GrowParams p) {
+  extern __shared__ int smem[];
+  int* const need = smem;
+  int* const first = need + p.slots;
+  int* const rank0 = first + p.slots;
+  int* const free_list = rank0 + p.slots;    // [pages]
+  sm100::launch_dependents();
+  sm100::grid_dependency_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = kGrowOneThreads / 32;
+  int free_all = 0, asked = 0;
+  each(threadIdx.x, p.pages, kGrowOneThreads, [&](int i) { return p.refs[i]; },
+       [&](int i, int r) { p.refs_out[i] = r; free_all += r <= 0; });
+  for (int b = warp; b < p.slots; b += warps) {
+    int lacks, at;
+    look_at_row(p, b, lacks, at);
+    if (lane == 0) { need[b] = lacks; first[b] = at; asked += lacks; }
+  }
+  free_all = block_sum(free_all);
+  asked = block_sum(asked);
+  rank_rows(p, rank0, asked, free_all, [&](int b) { return need[b]; });
+  enumerate(0, p.pages, 0, asked, [&](int i) { return p.refs[i]; }, [](int r) { return r <= 0; },
+            [&](int i, int rank) { free_list[rank] = i; });
+  __syncthreads();
+  for (int b = warp; b < p.slots; b += warps)
+    give(p, b, need[b], first[b], (int)min((long long)p.width, pages_wanted(p, b)), rank0[b], free_all,
+         [&](int i) { return free_list[i]; });
 }
 
 // ---------------------------------------------------------------------------- forking
@@ -398,56 +466,208 @@ __global__ void __launch_bounds__(kPlanThreads, 1) compact_kernel(const CompactP
 
 // ---------------------------------------------------------------------------- copies
 constexpr int kCopyPools = 128;          // pools one launch takes (its parameters stay below 4 KB)
-constexpr int kCopyThreads = 256;
-constexpr int kCopyUnit = 16384;         // bytes of a page that a CTA moves at a time
+constexpr int kCopyThreads = 512;
+constexpr int kTeam = 256;               // threads that move a unit, 128 bytes each at a time
+constexpr int kCopyUnit = 32768;         // bytes
 
-struct CopyParams {
-  const int* count;
-  const int* src;
-  const int* dst;
+struct CopyPools {
   int n_pools;
   int unit0[kCopyPools + 1];             // units of a page in the pools before this one
   b200attn_page_pool pools[kCopyPools];
 };
+struct CopyParams {
+  const int* count;
+  const int* src;
+  const int* dst;
+  CopyPools to;
+};
 
 template <typename V>
 __device__ __forceinline__ void copy_unit(const char* src, char* dst, int bytes) {
-  constexpr int kPer = 4;
+  constexpr int kPer = 8;
   const V* s = reinterpret_cast<const V*>(src);
   V* d = reinterpret_cast<V*>(dst);
-  const int n = bytes / (int)sizeof(V);
-  for (int i0 = threadIdx.x; i0 < n; i0 += kPer * kCopyThreads) {
+  const int n = bytes / (int)sizeof(V), tid = threadIdx.x % kTeam;
+  for (int i0 = tid; i0 < n; i0 += kPer * kTeam) {
     V v[kPer];
 #pragma unroll
     for (int j = 0; j < kPer; ++j)
-      if (i0 + j * kCopyThreads < n) v[j] = s[i0 + j * kCopyThreads];
+      if (i0 + j * kTeam < n) v[j] = __ldcs(s + i0 + j * kTeam);
 #pragma unroll
     for (int j = 0; j < kPer; ++j)
-      if (i0 + j * kCopyThreads < n) d[i0 + j * kCopyThreads] = v[j];
+      if (i0 + j * kTeam < n) __stcs(d + i0 + j * kTeam, v[j]);
+  }
+}
+// This CTA's share of: pool[dst[i]] = pool[src[i]] for i < count and every pool.  No page is both a source
+// and a destination.
+__device__ __forceinline__ void copy_share(const CopyPools& to, int count, const int* src, const int* dst) {
+  const int each = to.unit0[to.n_pools];
+  const long long units = (long long)count * each;
+  constexpr int kTeams = kCopyThreads / kTeam;
+  for (long long u = blockIdx.x * kTeams + threadIdx.x / kTeam; u < units; u += gridDim.x * kTeams) {
+    const int copy = (int)(u / each), unit = (int)(u % each);
+    int a = 0, b = to.n_pools;           // the pool with unit0[a] <= unit < unit0[a + 1]
+    while (b - a > 1) {
+      const int m = (a + b) >> 1;
+      if (to.unit0[m] <= unit) a = m; else b = m;
+    }
+    const b200attn_page_pool& pool = to.pools[a];
+    const long long off = (long long)(unit - to.unit0[a]) * kCopyUnit;
+    const int bytes = (int)min((long long)kCopyUnit, (long long)pool.page_bytes - off);
+    const char* from = (const char*)pool.base + src[copy] * (long long)pool.stride_bytes + off;
+    char* at = (char*)pool.base + dst[copy] * (long long)pool.stride_bytes + off;
+    if ((((uintptr_t)pool.base | pool.stride_bytes | pool.page_bytes) & 15) == 0) copy_unit<uint4>(from, at, bytes);
+    else copy_unit<unsigned>(from, at, bytes);
   }
 }
 
-// pool[dst[i]] = pool[src[i]] for every pool; no page is both a source and a destination.
-__global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const __grid_constant__ CopyParams p) {
+__global__ void __launch_bounds__(kCopyThreads, 2) copy_pages_kernel(const __grid_constant__ CopyParams p) {
   sm100::launch_dependents();
   sm100::grid_dependency_wait();
-  const int each = p.unit0[p.n_pools];
-  const long long units = (long long)*p.count * each;
-  for (long long u = blockIdx.x; u < units; u += gridDim.x) {
-    const int copy = (int)(u / each), unit = (int)(u % each);
-    int a = 0, b = p.n_pools;            // the pool with unit0[a] <= unit < unit0[a + 1]
-    while (b - a > 1) {
-      const int m = (a + b) >> 1;
-      if (p.unit0[m] <= unit) a = m; else b = m;
-    }
-    const b200attn_page_pool& pool = p.pools[a];
-    const long long off = (long long)(unit - p.unit0[a]) * kCopyUnit;
-    const int bytes = (int)min((long long)kCopyUnit, (long long)pool.page_bytes - off);
-    const char* src = (const char*)pool.base + p.src[copy] * (long long)pool.stride_bytes + off;
-    char* dst = (char*)pool.base + p.dst[copy] * (long long)pool.stride_bytes + off;
-    if ((((uintptr_t)pool.base | pool.stride_bytes | pool.page_bytes) & 15) == 0) copy_unit<uint4>(src, dst, bytes);
-    else copy_unit<unsigned>(src, dst, bytes);
+  copy_share(p.to, *p.count, p.src, p.dst);
+}
+
+// ---------------------------------------------------------------------------- both in one launch
+struct ForkCopyParams {
+  ForkParams book;
+  int books;                             // this launch writes the tables (the others copy further pools)
+  CopyPools to;
+};
+
+__global__ void __launch_bounds__(kCopyThreads, 2) fork_copy_kernel(const __grid_constant__ ForkCopyParams q) {
+  extern __shared__ int smem[];
+  const ForkParams& p = q.book;
+  int* const count = smem;               // [pages] rows that hold a page
+  int* const keeper = count + p.pages;   // [slots] the slot that has the row of this one whole; then number of the slot's copy
+  int* const lens = keeper + p.slots;    // [slots]
+  int* const from = lens + p.slots;      // [slots] its parent, kFreed or kStays
+  int* const upto = from + p.slots;      // [slots] entries it shares (all: INT_MAX)
+  int* const last = upto + p.slots;      // [slots] the entry it needs a copy of, or -1
+  int* const want = last + p.slots;      // [slots] the page there, or -1
+  int* const src = want + p.slots;       // [slots]
+  int* const dst = src + p.slots;
+  constexpr int kFreed = -1, kStays = -2;
+  sm100::launch_dependents();
+  const int tid = threadIdx.x;
+  for (int b = tid; b < p.slots; b += kCopyThreads) { keeper[b] = INT_MAX; want[b] = -1; }
+  __syncthreads();
+  sm100::grid_dependency_wait();
+  each(tid, p.slots, kCopyThreads, [&](int b) { return p.lens[b]; },
+       [&](int b, int n) { lens[b] = (int)min((long long)max(n, 0), (long long)p.width * p.page_size); });
+  each(tid, p.slots, kCopyThreads, [&](int b) { return p.parents[b]; }, [&](int b, int parent) {
+    const bool alive = parent >= 0 && parent < p.slots;
+    from[b] = !alive ? kFreed : parent == b ? kStays : parent;
+    if (alive) atomicMin(&keeper[parent], parent == b ? -1 : b);
+  });
+  each(tid, p.pages, kCopyThreads, [&](int i) { return p.refs[i]; }, [&](int i, int r) { count[i] = r; });
+  __syncthreads();
+  auto length = [&](int b) -> int {      // of the sequence that slot b becomes
+    const int parent = from[b] == kStays ? b : from[b];
+    return parent < 0 ? 0 : lens[parent];
+  };
+  for (int b = tid; b < p.slots; b += kCopyThreads) {
+    const int len = length(b), full = len / p.page_size;
+    const bool keeps = from[b] == kStays || (from[b] >= 0 && keeper[from[b]] == b);
+    upto[b] = keeps ? INT_MAX : full;
+    last[b] = !keeps && len % p.page_size ? full : -1;
   }
+  __syncthreads();
+  // rows let go and taken, the entries of both asked for together
+  const int warp = tid >> 5, warps = kCopyThreads / 32, lane = tid & 31;
+  auto inherited = [&](int b, int i) -> int {   // an entry of the row that slot b becomes
+    const int parent = from[b];
+    return parent == kFreed ? -1 : p.table[(long long)(parent == kStays ? b : parent) * p.width + i];
+  };
+  constexpr int kRows = kAhead / 2;
+  for (int b0 = warp * kRows; b0 < p.slots; b0 += warps * kRows)
+    for (int i = lane; i < p.width; i += 32) {
+      int gone[kRows], taken[kRows];
+#pragma unroll
+      for (int j = 0; j < kRows; ++j) {
+        const bool moves = b0 + j < p.slots && from[b0 + j] != kStays;
+        gone[j] = moves ? p.table[(long long)(b0 + j) * p.width + i] : -1;
+        taken[j] = moves ? inherited(b0 + j, i) : -1;
+      }
+#pragma unroll
+      for (int j = 0; j < kRows; ++j) {
+        if (gone[j] >= 0 && gone[j] < p.pages) atomicSub(&count[gone[j]], 1);
+        if (taken[j] < 0 || taken[j] >= p.pages) continue;
+        if (i < upto[b0 + j]) atomicAdd(&count[taken[j]], 1);
+        else if (i == last[b0 + j]) want[b0 + j] = taken[j];
+      }
+    }
+  __syncthreads();
+  int* const place = keeper;
+  const int asked = enumerate(0, p.slots, 0, INT_MAX, [&](int b) { return want[b]; }, [](int e) { return e >= 0; },
+            [&](int b, int rank) { src[rank] = want[b]; place[b] = rank; });
+  // (the count of a page handed out is set behind the enumeration, which reads the counts)
+  const int given = min(asked, enumerate(0, p.pages, 0, asked, [&](int i) { return count[i]; },
+                                         [](int r) { return r <= 0; }, [&](int i, int rank) { dst[rank] = i; }));
+  __syncthreads();
+  for (int i = tid; i < given; i += kCopyThreads) count[dst[i]] = 1;
+  __syncthreads();
+  if (q.books) {                         // this CTA's share of the new tables
+    const int at0 = blockIdx.x * kCopyThreads + tid, step = gridDim.x * kCopyThreads;
+    each_entry(p.slots, p.width, blockIdx.x * warps + warp, gridDim.x * warps, inherited, [&](int b, int i, int e) {
+      int taken = e >= 0 && e < p.pages && i < upto[b] ? e : -1;
+      if (i == last[b] && want[b] >= 0 && place[b] < given) taken = dst[place[b]];
+      p.table_out[(long long)b * p.width + i] = taken;
+    });
+    for (int b = at0; b < p.slots; b += step) {
+      const int len = length(b);
+      p.lens_out[b] = want[b] >= 0 && place[b] >= given ? len / p.page_size * p.page_size : len;
+    }
+    for (int i = at0; i < p.pages; i += step) p.refs_out[i] = count[i];
+    if (blockIdx.x == 0 && tid == 0) *p.missing = asked - given;
+  }
+  copy_share(q.to, given, src, dst);
+}
+
+struct CompactCopyParams {
+  CompactParams book;
+  int books;
+  CopyPools to;
+};
+
+__global__ void __launch_bounds__(kCopyThreads, 2) compact_copy_kernel(const __grid_constant__ CompactCopyParams q) {
+  extern __shared__ int smem[];
+  const CompactParams& p = q.book;
+  constexpr int kStays = -1, kFree = -2;
+  int* const what = smem;                // [pages] kStays, kFree, or the page a moving one goes to, or that a free place gets
+  int* const src = what + p.pages;       // [pages / 2 + 1]
+  int* const dst = src + p.pages / 2 + 1;
+  sm100::launch_dependents();
+  sm100::grid_dependency_wait();
+  const int tid = threadIdx.x;
+  int n = 0;
+  each(tid, p.pages, kCopyThreads, [&](int i) { return p.refs[i]; }, [&](int i, int r) {
+    what[i] = r > 0 ? kStays : kFree;
+    n += r > 0;
+  });
+  n = block_sum(n);                      // (also the barrier in front of the reads)
+  auto state = [&](int i) { return what[i]; };
+  const int moves = enumerate(0, n, 0, INT_MAX, state, [](int w) { return w == kFree; }, [&](int i, int rank) { dst[rank] = i; });
+  enumerate(n, p.pages, 0, INT_MAX, state, [](int w) { return w == kStays; }, [&](int i, int rank) { src[rank] = i; });
+  __syncthreads();
+  for (int i = tid; i < moves; i += kCopyThreads) {
+    what[src[i]] = dst[i];
+    what[dst[i]] = src[i];
+  }
+  __syncthreads();
+  if (q.books) {                         // this CTA's share of the new tables
+    const int at = blockIdx.x * kCopyThreads + tid, step = gridDim.x * kCopyThreads;
+    for (int i = at; i < p.pages; i += step) p.refs_out[i] = i < n ? p.refs[what[i] == kStays ? i : what[i]] : 0;
+    each(at, p.slots * p.width, step, [&](int i) { return p.table[i]; }, [&](int i, int e) {
+      int to = -1;
+      if (e >= 0 && e < p.pages) {
+        if (e < n) to = what[e] == kStays ? e : -1;
+        else to = what[e] >= 0 ? what[e] : -1;
+      }
+      p.table_out[i] = to;
+    });
+    if (blockIdx.x == 0 && tid == 0) *p.live = n;
+  }
+  copy_share(q.to, moves, src, dst);
 }
 
 // ---------------------------------------------------------------------------- host side
@@ -470,6 +690,7 @@ int check_book(const int32_t* table, const int32_t* refs, const int32_t* table_o
 }
 
 int check_workspace(const void* ws, size_t bytes, size_t need) {
+  if (need == 0) return B200ATTN_OK;
   if (!ws || bytes < need) return B200ATTN_ERR_WORKSPACE;
   return ((uintptr_t)ws & 15) ? B200ATTN_ERR_ALIGN : B200ATTN_OK;
 }
@@ -487,13 +708,12 @@ int check_pools(const b200attn_page_pool* pools, int n) {
 }
 
 template <typename P>
-int launch_plan(void (*kernel)(P), const P& p, long long entries, size_t smem, cudaStream_t stream) {
+int launch_plan(void (*kernel)(P), const P& p, size_t smem, cudaStream_t stream) {
   if (smem > 48 * 1024 &&
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
     return B200ATTN_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
-  const int ctas = entries <= kOneCta ? 1 : kPlanCtas;
-  cfg.gridDim = dim3(ctas);
+  cfg.gridDim = dim3(kPlanCtas);
   cfg.blockDim = dim3(kPlanThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -501,11 +721,24 @@ int launch_plan(void (*kernel)(P), const P& p, long long entries, size_t smem, c
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = ctas;
+  attr[1].val.clusterDim.x = kPlanCtas;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
   return cudaLaunchKernelEx(&cfg, kernel, p) == cudaSuccess ? B200ATTN_OK : B200ATTN_ERR_CUDA;
+}
+
+// Pools [at, at + kCopyPools) of the caller's.
+int pools_of(const b200attn_page_pool* pools, int n_pools, int at, CopyPools& to) {
+  to.n_pools = std::min(kCopyPools, n_pools - at);
+  to.unit0[0] = 0;
+  for (int i = 0; i < to.n_pools; ++i) {
+    to.pools[i] = pools[at + i];
+    const long long units = to.unit0[i] + (pools[at + i].page_bytes + kCopyUnit - 1) / kCopyUnit;
+    if (units > INT_MAX) return B200ATTN_ERR_TOO_LARGE;
+    to.unit0[i + 1] = (int)units;
+  }
+  return B200ATTN_OK;
 }
 
 // The copies of the list in the workspace, kCopyPools pools a launch; `launches` counts them.
@@ -514,25 +747,46 @@ int launch_copies(const b200attn_page_pool* pools, int n_pools, const int* count
   for (int at = 0; at < n_pools; at += kCopyPools) {
     CopyParams p;
     p.count = count; p.src = src; p.dst = dst;
-    p.n_pools = std::min(kCopyPools, n_pools - at);
-    p.unit0[0] = 0;
-    for (int i = 0; i < p.n_pools; ++i) {
-      p.pools[i] = pools[at + i];
-      const long long units = p.unit0[i] + (pools[at + i].page_bytes + kCopyUnit - 1) / kCopyUnit;
-      if (units > INT_MAX) return B200ATTN_ERR_TOO_LARGE;
-      p.unit0[i + 1] = (int)units;
-    }
-    if (launch_after(copy_pages_kernel, dim3(sm_count * 8), dim3(kCopyThreads), 0, stream, p) != cudaSuccess)
+    if (int st = pools_of(pools, n_pools, at, p.to)) return st;
+    if (launch_after(copy_pages_kernel, dim3(sm_count * 2), dim3(kCopyThreads), 0, stream, p) != cudaSuccess)
       return B200ATTN_ERR_CUDA;
     ++launches;
   }
   return B200ATTN_OK;
 }
 
+// Books and copies in one kernel, again for every kCopyPools pools (once without any).
+template <typename P, typename B>
+int launch_both(void (*kernel)(P), const B& book, size_t smem, const b200attn_page_pool* pools, int n_pools, int sm_count,
+                cudaStream_t stream, int& launches) {
+  if (smem > 48 * 1024 &&
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    return B200ATTN_ERR_CUDA;
+  for (int at = 0; at == 0 || at < n_pools; at += kCopyPools) {
+    P p;
+    p.book = book;
+    p.books = at == 0;
+    if (int st = pools_of(pools, n_pools, at, p.to)) return st;
+    if (launch_after(kernel, dim3(sm_count * 2), dim3(kCopyThreads), smem, stream, p) != cudaSuccess) return B200ATTN_ERR_CUDA;
+    ++launches;
+  }
+  return B200ATTN_OK;
+}
+// Shared memory with which two CTAs fit an SM.
+constexpr size_t kBothSmem = 112 * 1024;
+size_t fork_smem(long long pages, long long slots) { return 4 * (size_t)(pages + 8 * slots); }
+size_t compact_smem(long long pages) { return 4 * (size_t)(pages + 2 * (pages / 2 + 1)); }
+
+// one CTA with its lists in shared memory
+bool grow_by_one(const b200attn_pages_grow_args* a) {
+  return (long long)a->slots * a->max_pages_per_seq + a->num_pages <= kGrowOneEntries &&
+         3LL * a->slots + a->num_pages <= kGrowOneInts;
+}
+
 }  // namespace
 
 size_t pages_grow_workspace_bytes(const b200attn_pages_grow_args* a) {
-  if (!a || a->slots <= 0 || a->num_pages <= 0) return 0;
+  if (!a || a->slots <= 0 || a->num_pages <= 0 || a->max_pages_per_seq <= 0 || grow_by_one(a)) return 0;
   return 4 * ((size_t)kHeader + 3 * (size_t)a->slots + a->num_pages);
 }
 
@@ -549,19 +803,25 @@ int pages_grow(const b200attn_pages_grow_args* a, cudaStream_t stream) {
   p.table = a->page_table; p.lens = a->seqlens; p.refs = a->page_refs; p.fresh = a->new_tokens;
   p.table_out = a->page_table_out; p.refs_out = a->page_refs_out; p.missing = a->missing_out;
   p.slots = a->slots; p.width = a->max_pages_per_seq; p.pages = a->num_pages; p.page_size = a->page_size;
+  if (grow_by_one(a)) {
+    const size_t smem = 4 * (3 * (size_t)a->slots + a->num_pages);
+    if (launch_after(grow_one_kernel, dim3(1), dim3(kGrowOneThreads), smem, stream, p) != cudaSuccess) return B200ATTN_ERR_CUDA;
+    set_launch_count(1);
+    return cudaGetLastError() == cudaSuccess ? B200ATTN_OK : B200ATTN_ERR_CUDA;
+  }
   p.header = (int*)a->workspace;
   p.need = p.header + kHeader;
   p.first = p.need + a->slots;
   p.rank0 = p.first + a->slots;
   p.free_list = p.rank0 + a->slots;
-  st = launch_plan(grow_kernel, p, (long long)p.slots * p.width + p.pages, 0, stream);
+  st = launch_plan(grow_kernel, p, 0, stream);
   if (st != B200ATTN_OK) return st;
   set_launch_count(1);
   return cudaGetLastError() == cudaSuccess ? B200ATTN_OK : B200ATTN_ERR_CUDA;
 }
 
 size_t pages_fork_workspace_bytes(const b200attn_pages_fork_args* a) {
-  if (!a || a->slots <= 0) return 0;
+  if (!a || a->slots <= 0 || a->num_pages <= 0 || fork_smem(a->num_pages, a->slots) <= kBothSmem) return 0;
   return 4 * ((size_t)kHeader + 4 * (size_t)a->slots);
 }
 
@@ -585,14 +845,22 @@ int pages_fork(const b200attn_pages_fork_args* a, cudaStream_t stream) {
   p.table_out = a->page_table_out; p.lens_out = a->seqlens_out; p.refs_out = a->page_refs_out;
   p.missing = a->missing_out;
   p.slots = a->slots; p.width = a->max_pages_per_seq; p.pages = a->num_pages; p.page_size = a->page_size;
+  int launches = 0;
+  const size_t smem = fork_smem(a->num_pages, a->slots);
+  if (smem <= kBothSmem) {
+    st = launch_both(fork_copy_kernel, p, smem, a->pools, a->n_pools, di->sm_count, stream, launches);
+    if (st != B200ATTN_OK) return st;
+    set_launch_count(launches);
+    return cudaGetLastError() == cudaSuccess ? B200ATTN_OK : B200ATTN_ERR_CUDA;
+  }
   p.header = (int*)a->workspace;
   p.want = p.header + kHeader;
   p.free_list = p.want + a->slots;
   p.src = p.free_list + a->slots;
   p.dst = p.src + a->slots;
-  st = launch_plan(fork_kernel, p, (long long)p.slots * p.width + p.pages, n, stream);
+  st = launch_plan(fork_kernel, p, n, stream);
   if (st != B200ATTN_OK) return st;
-  int launches = 1;
+  launches = 1;
   st = launch_copies(a->pools, a->n_pools, p.header + kCopies, p.src, p.dst, di->sm_count, stream, launches);
   if (st != B200ATTN_OK) return st;
   set_launch_count(launches);
@@ -600,7 +868,7 @@ int pages_fork(const b200attn_pages_fork_args* a, cudaStream_t stream) {
 }
 
 size_t pages_compact_workspace_bytes(const b200attn_pages_compact_args* a) {
-  if (!a || a->num_pages <= 0) return 0;
+  if (!a || a->num_pages <= 0 || compact_smem(a->num_pages) <= kBothSmem) return 0;
   return 4 * ((size_t)kHeader + 3 * (size_t)a->num_pages);
 }
 
@@ -619,13 +887,21 @@ int pages_compact(const b200attn_pages_compact_args* a, cudaStream_t stream) {
   p.table = a->page_table; p.refs = a->page_refs;
   p.table_out = a->page_table_out; p.refs_out = a->page_refs_out; p.live = a->live_out;
   p.slots = a->slots; p.width = a->max_pages_per_seq; p.pages = a->num_pages;
+  int launches = 0;
+  const size_t smem = compact_smem(a->num_pages);
+  if (smem <= kBothSmem) {
+    st = launch_both(compact_copy_kernel, p, smem, a->pools, a->n_pools, di->sm_count, stream, launches);
+    if (st != B200ATTN_OK) return st;
+    set_launch_count(launches);
+    return cudaGetLastError() == cudaSuccess ? B200ATTN_OK : B200ATTN_ERR_CUDA;
+  }
   p.header = (int*)a->workspace;
   p.rank_of = p.header + kHeader;
   p.src = p.rank_of + a->num_pages;
   p.dst = p.src + a->num_pages;
-  st = launch_plan(compact_kernel, p, (long long)p.slots * p.width + p.pages, 0, stream);
+  st = launch_plan(compact_kernel, p, 0, stream);
   if (st != B200ATTN_OK) return st;
-  int launches = 1;
+  launches = 1;
   st = launch_copies(a->pools, a->n_pools, p.header + kCopies, p.src, p.dst, di->sm_count, stream, launches);
   if (st != B200ATTN_OK) return st;
   set_launch_count(launches);
