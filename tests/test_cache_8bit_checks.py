@@ -43,7 +43,7 @@ def decode_args():
     a.workspace_bytes = 1 << 40
     a.dtype, a.cache_dtype, a.batch, a.queries = 1, 3, 2, 1
     a.heads_q, a.heads_kv, a.head_dim = 8, 2, 128
-    a.page_size, a.block_tokens, a.num_pages, a.max_pages_per_seq, a.max_seqlen = 64, 16, 10, 4, 256
+    a.page_size, a.block_tokens, a.num_pages, a.max_pages_per_seq, a.max_seqlen = 64, 16, 10, 400, 25600
     return a
 
 

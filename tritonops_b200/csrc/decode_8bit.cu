@@ -774,9 +774,10 @@ long long rows_of(const b200attn_paged_decode_8bit_args* a) {
   return (long long)a->queries * (a->heads_q / a->heads_kv);
 }
 
-// Split size: the one with the least waves x (stages of a chunk + 4) + half a chunk + 3 where there is
+// Split size: the one with the least waves x (stages of a chunk + 4) + half a chunk + 4 where there is
 // more than one chunk, all lengths taken as the largest.  Four stages are a chunk's own cost (look-ups
-// behind a full ring, the fold), half a chunk the uneven end of a ragged batch, three the second kernel.
+// behind a full ring, the fold), half a chunk the uneven end of a ragged batch, four the second kernel
+// and its launch.
 // Measured on B200, 8 KV heads, D = 128, us: 64 sequences of 4096 keys 90.5 in one chunk, 96 in 1024; of
 // 1024-8192 118.7 in 2048, 125 in 1024, 132 in one; 16 of 1024-8192 47.3 in 2048, 44.0 in 1536, 49.6 in
 // 4096; 12 of 4096 26.0 in 1536, 28.6 in 2048; 8 of 2048 13.5 in 512, 15.3 in 768; four of 90001-131072
@@ -789,7 +790,7 @@ int chunk_of(const b200attn_paged_decode_8bit_args* a) {
   long long best = 0, least = 0;
   auto consider = [&](long long per) {
     const long long n = (stages + per - 1) / per;
-    const long long cost = 2 * ((units * n + kSlots - 1) / kSlots) * (per + 4) + per + (n > 1 ? 6 : 0);
+    const long long cost = 2 * ((units * n + kSlots - 1) / kSlots) * (per + 4) + per + (n > 1 ? 8 : 0);
     if (!best || cost < least) { best = per; least = cost; }
   };
   const int sizes[10] = {1, 2, 3, 4, 6, 8, 12, 16, 32, 64};
@@ -872,7 +873,7 @@ int launch(const b200attn_paged_decode_8bit_args* a, const Decode8Params& p, dim
 size_t paged_decode_8bit_workspace_bytes(const b200attn_paged_decode_8bit_args* a) {
   if (!a || a->batch <= 0 || a->queries <= 0 || a->heads_q <= 0 || a->heads_kv <= 0 || a->head_dim <= 0) return 0;
   const long long chunks = chunks_of(a);
-  if (chunks == 1) return 16;          // phase 1 writes the result itself
+  if (chunks == 1) return 0;           // phase 1 writes the result itself
   const size_t rows = (size_t)a->batch * a->queries * a->heads_q * chunks;
   return rows * a->head_dim * 4 + rows * 4;
 }
@@ -883,7 +884,8 @@ int paged_decode_8bit_fwd(const b200attn_paged_decode_8bit_args* a, cudaStream_t
   const long long rows = rows_of(a), tiles = (rows + kRowsTile - 1) / kRowsTile;
   const long long chunks = chunks_of(a);
   if (a->heads_kv * rows > INT_MAX || chunks > 65535 || max_visible(a) > INT_MAX - 65536) return B200ATTN_ERR_TOO_LARGE;
-  if (!a->workspace || a->workspace_bytes < paged_decode_8bit_workspace_bytes(a)) return B200ATTN_ERR_WORKSPACE;
+  if (const size_t need = paged_decode_8bit_workspace_bytes(a))
+    if (!a->workspace || a->workspace_bytes < need) return B200ATTN_ERR_WORKSPACE;
   if ((uintptr_t)a->workspace & 15) return B200ATTN_ERR_ALIGN;
   const DeviceInfo* di = nullptr;
   if ((st = device_info(&di)) != B200ATTN_OK) return st;

@@ -13,6 +13,8 @@
 #include <ATen/ATen.h>
 #include <ATen/TracerMode.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <dlfcn.h>
@@ -107,6 +109,14 @@ const int32_t* int_list(PyObject* o, const at::Tensor& like, at::Tensor* keep = 
 
 at::Tensor scratch(size_t bytes, const at::Tensor& like) {
   return at::empty({(int64_t)std::max<size_t>(bytes, 16)}, like.options().dtype(at::kByte).requires_grad(false));
+}
+// scratch of the page operators and of the 8-bit cache: memory without a tensor around it
+c10::DataPtr scratch_memory(size_t bytes) {
+  return c10::cuda::CUDACachingAllocator::get()->allocate(bytes);
+}
+// a tensor of the current device, without the dispatcher
+at::Tensor made(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& like) {
+  return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
 }
 at::Tensor fresh(at::IntArrayRef sizes, const at::Tensor& like) {
   return at::empty(sizes, like.options().requires_grad(false));
@@ -383,12 +393,15 @@ PyObject* paged_decode_8bit(PyObject*, PyObject* const* x, Py_ssize_t n) {
     a.softmax_scale = x[8] == Py_None ? (float)std::pow((double)a.head_dim, -0.5) : real(x[8]);
     a.chunk_tokens = int32(x[9]);
     const c10::cuda::CUDAGuard device(q.device());
-    at::Tensor o = fresh(q.sizes(), q);
+    at::Tensor o = made(q.sizes(), q.scalar_type(), q);
     a.q = q.data_ptr(); a.o = o.data_ptr();
     a.q_stride_b = q.stride(0); a.q_stride_t = dim == 4 ? q.stride(1) : 0; a.q_stride_h = q.stride(dim - 2);
     a.o_stride_b = o.stride(0); a.o_stride_t = dim == 4 ? o.stride(1) : 0; a.o_stride_h = o.stride(dim - 2);
-    at::Tensor ws = scratch(L.paged_decode_8bit_workspace_bytes(&a), q);
-    a.workspace = ws.data_ptr(); a.workspace_bytes = (size_t)ws.numel();
+    c10::DataPtr ws;
+    if ((a.workspace_bytes = L.paged_decode_8bit_workspace_bytes(&a))) {
+      ws = scratch_memory(a.workspace_bytes);
+      a.workspace = ws.get();
+    }
     long long launches;
     const int st = call(L.paged_decode_8bit_fwd, a, q, launches);
     return answer(st, launches, {o});
@@ -434,7 +447,7 @@ const int32_t* per_slot(PyObject* o, const at::Tensor& table, at::Tensor& t) {
   need(p && t.numel() == table.size(0));
   return p;
 }
-at::Tensor one_int(const at::Tensor& like) { return at::empty({1}, like.options().requires_grad(false)); }
+at::Tensor ints(at::IntArrayRef sizes, const at::Tensor& like) { return made(sizes, at::kInt, like); }
 
 // tensors [num_pages, ...] whose pages are contiguous
 std::vector<b200attn_page_pool> page_pools(PyObject* list, const at::Tensor& refs) {
@@ -468,13 +481,13 @@ PyObject* grow_pages(PyObject*, PyObject* const* x, Py_ssize_t n) {
     a.seqlens = per_slot(x[1], table, lens); a.new_tokens = per_slot(x[3], table, more);
     a.page_size = int32(x[4]);
     const c10::cuda::CUDAGuard device(table.device());
-    at::Tensor out = fresh(table.sizes(), table), refs_out = fresh(refs.sizes(), refs), missing = one_int(refs);
+    at::Tensor out = ints(table.sizes(), table), refs_out = ints(refs.sizes(), refs), missing = ints({1}, refs);
     a.page_table_out = out.data_ptr<int32_t>(); a.page_refs_out = refs_out.data_ptr<int32_t>();
     a.missing_out = missing.data_ptr<int32_t>();
-    at::Tensor ws;
-    if (const size_t bytes = L.pages_grow_workspace_bytes(&a)) {
-      ws = scratch(bytes, table);
-      a.workspace = ws.data_ptr(); a.workspace_bytes = (size_t)ws.numel();
+    c10::DataPtr ws;
+    if ((a.workspace_bytes = L.pages_grow_workspace_bytes(&a))) {
+      ws = scratch_memory(a.workspace_bytes);
+      a.workspace = ws.get();
     }
     long long launches;
     const int st = call(L.pages_grow, a, table, launches);
@@ -493,14 +506,14 @@ PyObject* fork_pages(PyObject*, PyObject* const* x, Py_ssize_t n) {
     const std::vector<b200attn_page_pool> pools = page_pools(x[0], refs);
     a.pools = pools.data(); a.n_pools = (int)pools.size();
     const c10::cuda::CUDAGuard device(table.device());
-    at::Tensor out = fresh(table.sizes(), table), refs_out = fresh(refs.sizes(), refs), missing = one_int(refs),
-               lens_out = fresh(lens.sizes(), lens);
+    at::Tensor out = ints(table.sizes(), table), refs_out = ints(refs.sizes(), refs), missing = ints({1}, refs),
+               lens_out = ints(lens.sizes(), lens);
     a.page_table_out = out.data_ptr<int32_t>(); a.page_refs_out = refs_out.data_ptr<int32_t>();
     a.seqlens_out = lens_out.data_ptr<int32_t>(); a.missing_out = missing.data_ptr<int32_t>();
-    at::Tensor ws;
-    if (const size_t bytes = L.pages_fork_workspace_bytes(&a)) {
-      ws = scratch(bytes, table);
-      a.workspace = ws.data_ptr(); a.workspace_bytes = (size_t)ws.numel();
+    c10::DataPtr ws;
+    if ((a.workspace_bytes = L.pages_fork_workspace_bytes(&a))) {
+      ws = scratch_memory(a.workspace_bytes);
+      a.workspace = ws.get();
     }
     long long launches;
     const int st = call(L.pages_fork, a, table, launches);
@@ -517,13 +530,13 @@ PyObject* compact_pages(PyObject*, PyObject* const* x, Py_ssize_t n) {
     const std::vector<b200attn_page_pool> pools = page_pools(x[0], refs);
     a.pools = pools.data(); a.n_pools = (int)pools.size();
     const c10::cuda::CUDAGuard device(table.device());
-    at::Tensor out = fresh(table.sizes(), table), refs_out = fresh(refs.sizes(), refs), live = one_int(refs);
+    at::Tensor out = ints(table.sizes(), table), refs_out = ints(refs.sizes(), refs), live = ints({1}, refs);
     a.page_table_out = out.data_ptr<int32_t>(); a.page_refs_out = refs_out.data_ptr<int32_t>();
     a.live_out = live.data_ptr<int32_t>();
-    at::Tensor ws;
-    if (const size_t bytes = L.pages_compact_workspace_bytes(&a)) {
-      ws = scratch(bytes, table);
-      a.workspace = ws.data_ptr(); a.workspace_bytes = (size_t)ws.numel();
+    c10::DataPtr ws;
+    if ((a.workspace_bytes = L.pages_compact_workspace_bytes(&a))) {
+      ws = scratch_memory(a.workspace_bytes);
+      a.workspace = ws.get();
     }
     long long launches;
     const int st = call(L.pages_compact, a, table, launches);
