@@ -55,7 +55,19 @@ struct AppendBlock {
   int page, index;                 // page of the pool, block of the page
 };
 
-__device__ __forceinline__ unsigned max_abs16(unsigned m, unsigned x) { return __vmaxu2(m, x & 0x7fff7fffu); }
+// max(m, |x|) of two numbers; NaN stays
+template <typename T>
+__device__ __forceinline__ unsigned max_abs2(unsigned m, unsigned x);
+template <>
+__device__ __forceinline__ unsigned max_abs2<__half>(unsigned m, unsigned x) {
+  asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(m) : "r"(x & 0x7fff7fffu));
+  return m;
+}
+template <>
+__device__ __forceinline__ unsigned max_abs2<__nv_bfloat16>(unsigned m, unsigned x) {
+  asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(x & 0x7fff7fffu));
+  return m;
+}
 
 template <typename T>
 __device__ __forceinline__ float2 unpack2(unsigned x);
@@ -147,10 +159,12 @@ struct Scaling {
                       quantise4<kE4M3>(times(c.x), times(c.y), times(c.z), times(c.w), 1.f));
   }
 };
-__device__ __forceinline__ unsigned max_abs_of(const uint4& x) {
-  const unsigned m = max_abs16(max_abs16(max_abs16(x.x & 0x7fff7fffu, x.y), x.z), x.w);
-  return max(m & 0xffffu, m >> 16);
+template <typename T>
+__device__ __forceinline__ unsigned max_abs8(unsigned m, const uint4& x) {
+  return max_abs2<T>(max_abs2<T>(max_abs2<T>(max_abs2<T>(m, x.x), x.y), x.z), x.w);
 }
+// the larger of the two as 15 bits (which order as the numbers do, NaN above all)
+__device__ __forceinline__ unsigned larger(unsigned m) { return max(m & 0x7fffu, (m >> 16) & 0x7fffu); }
 
 // One new row for each sequence: a few kilobytes, so the time is the chain of look-ups (length, page,
 // scale).  A group of head_dim / 8 lanes takes the row of one (sequence, head, K or V), which it asks
@@ -177,7 +191,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_8bit_one_kernel(const A
                         (long long)index * p.block * p.page_st[which] + h * p.page_sh[which] + col;
   const unsigned group = (lanes == 32 ? 0xffffffffu : (1u << lanes) - 1u) << (mine * lanes);
   const float before = off ? *scale : 0.f;
-  const unsigned top = __reduce_max_sync(group, max_abs_of(x));
+  const unsigned top = __reduce_max_sync(group, larger(max_abs8<T>(0u, x)));
   const Scaling<T, kE4M3> sc(top, before);
   *reinterpret_cast<uint2*>(base + off * p.page_st[which]) = sc.pow2 ? sc.template eight<true>(x) : sc.template eight<false>(x);
   if (off && sc.after > before) {              // (eight rows' loads together: the others wait for this)
@@ -274,8 +288,8 @@ __global__ void __launch_bounds__(kAppendThreads, 2) append_8bit_kernel(const Ap
     unsigned top = 0;
     if (some) {
 #pragma unroll
-      for (int i = 0; i < kUnitRows / 2; ++i) top = max(top, max_abs_of(now.x[i]));
-      top = __reduce_max_sync(0xffffffffu, top);
+      for (int i = 0; i < kUnitRows / 2; ++i) top = max_abs8<T>(top, now.x[i]);
+      top = __reduce_max_sync(0xffffffffu, larger(top));
     }
     if (wpt > 1) {                             // the warps of a task meet (two sets of places, one barrier)
       if (lane == 0) tops[turn][warp] = top;
