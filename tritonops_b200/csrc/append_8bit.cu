@@ -12,8 +12,7 @@
 // move with every new maximum and round the block's int8 rows again each time).
 //
 // A task is one (block, head, K or V): the block's 16-row units go to a warp each, 16 bytes per lane
-// and row, stay in registers between the maximum and the rounding, and leave as 8-byte pieces.  The
-// CTA that holds a block's first new token does the whole block, so no two CTAs share a scale.
+// and row, stay in registers between the maximum and the rounding, and leave as 8-byte pieces.
 #include <limits.h>
 
 #include <algorithm>
@@ -28,7 +27,7 @@ namespace {
 constexpr int kAppendThreads = 256;
 constexpr int kAppendWarps = kAppendThreads / 32;
 constexpr int kCtasPerSm = 2;
-constexpr int kMaxBlockTokens = 128;
+constexpr int kListed = 128;                   // blocks a CTA looks up at a time
 constexpr int kUnitRows = 16;
 
 struct AppendParams {
@@ -43,17 +42,51 @@ struct AppendParams {
   const int32_t* cu;               // nullptr: token t is sequence t's only new one
   int tokens, batch, heads, head_dim;
   int page_size, block, num_pages, width;
-  int tile;                        // tokens whose blocks a CTA looks after
-  int warps_per_task;              // one for each 16-row unit of a block that can hold new rows
-  int jobs_per_cta;                // (head, K or V) pairs of a CTA
+  int warps_per_task;              // one for each 16-row unit of a block
 };
 
-// one block that begins to be written in the CTA's tile
+// one block that gets new rows
 struct AppendBlock {
-  int row0;                        // its first new row
-  int off, fresh;                  // tokens the block holds already, new ones
+  int row0;                        // the first of them
+  int off, fresh;                  // tokens the block holds already, new ones (none: its page is nowhere)
   int page, index;                 // page of the pool, block of the page
 };
+
+// the rows sequence i gets, as far as the table has room, and the blocks they fall into
+struct AppendRun {
+  int first, count, len, blocks;
+  __device__ __forceinline__ AppendRun(const AppendParams& p, int i) : first(0), count(0), len(0), blocks(0) {
+    if (i >= p.batch) return;
+    first = p.cu[i];
+    const int end = min(p.cu[i + 1], p.tokens);
+    len = p.lens[i];
+    if (first < 0 || first >= end || len < 0) return;
+    count = (int)max(0ll, min((long long)(end - first), (long long)p.width * p.page_size - len));
+    if (count > 0) blocks = (int)(((long long)(len & (p.block - 1)) + count + p.block - 1) / p.block);
+  }
+};
+
+// sum of n over the CTA's threads before this one, and over all of them
+__device__ __forceinline__ long long sum_before(long long n, long long* sums, long long& all) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long upto = n;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long other = __shfl_up_sync(0xffffffffu, upto, d);
+    if (lane >= d) upto += other;
+  }
+  __syncthreads();
+  if (lane == 31) sums[warp] = upto;
+  __syncthreads();
+  long long before = upto - n;
+  all = 0;
+#pragma unroll
+  for (int i = 0; i < kAppendWarps; ++i) {
+    if (i < warp) before += sums[i];
+    all += sums[i];
+  }
+  return before;
+}
 
 // max(m, |x|) of two numbers; NaN stays
 template <typename T>
@@ -209,129 +242,147 @@ __global__ void __launch_bounds__(kAppendThreads) append_8bit_one_kernel(const A
   if (col == 0) *scale = sc.after;
 }
 
-// Packed new rows.  The loads of the next task are under way while a warp works on one.
+// Packed new rows.  The tasks of all sequences form one list, of which each CTA takes an equal share.  The
+// loads of the next task are under way while a warp works on one.
 template <typename T, bool kE4M3>
-__global__ void __launch_bounds__(kAppendThreads, 2) append_8bit_kernel(const AppendParams p) {
-  __shared__ AppendBlock blocks[kMaxBlockTokens];
-  __shared__ int n_blocks;
+__global__ void __launch_bounds__(kAppendThreads, kCtasPerSm) append_8bit_kernel(const AppendParams p) {
+  __shared__ AppendBlock blocks[kListed];
+  __shared__ int owner[kListed];               // sequence of a listed block
+  __shared__ int nth[kListed];                 // which of the sequence's blocks it is
+  __shared__ long long sums[kAppendWarps], share[2];
   __shared__ unsigned tops[2][kAppendWarps];
   sm100::launch_dependents();
-  if (threadIdx.x == 0) n_blocks = 0;
   sm100::grid_dependency_wait();
-  // ---- which blocks begin to be written in this tile
-  const int t0 = blockIdx.x * p.tile;
-  int b = 0;                                   // sequences that end at or before t0
-  for (int i0 = 0; i0 < p.batch; i0 += kAppendThreads) {
-    const int i = i0 + threadIdx.x;
-    b += __syncthreads_count(i < p.batch && p.cu[i + 1] <= t0);
+  const int n_jobs = 2 * p.heads;
+  long long list0;                             // the first block of the list (of all sequences' blocks)
+  {
+    long long total = 0, all;
+    for (int i0 = 0; i0 < p.batch; i0 += kAppendThreads) {
+      sum_before(AppendRun(p, i0 + threadIdx.x).blocks, sums, all);
+      total += all;
+    }
+    if (total > p.tokens / p.block + 2ll * p.batch) return;     // (not ascending: rows of more sequences than one)
+    total *= n_jobs;
+    list0 = total * blockIdx.x / gridDim.x / n_jobs;
+    if (threadIdx.x == 0) {
+      share[0] = total * blockIdx.x / gridDim.x;
+      share[1] = total * (blockIdx.x + 1) / gridDim.x;
+    }
+    __syncthreads();
+  }
+  for (int turn = 0; list0 * n_jobs < share[1]; list0 += kListed) {
+  // ---- look the blocks up
+  const int n_listed = (int)min((long long)kListed, (share[1] + n_jobs - 1) / n_jobs - list0);
+  long long at = -list0;
+  for (int i0 = 0; i0 < p.batch && at < n_listed; i0 += kAppendThreads) {
+    const AppendRun run(p, i0 + threadIdx.x);
+    long long all;
+    const long long mine = at + sum_before(run.blocks, sums, all);
+    const int end = (int)min((long long)n_listed, mine + run.blocks);
+    for (int j = (int)max(0ll, mine); j < end; ++j) {
+      owner[j] = i0 + threadIdx.x;
+      nth[j] = (int)(j - mine);
+    }
+    at += all;
   }
   __syncthreads();
-  const int t = t0 + threadIdx.x;
-  if ((int)threadIdx.x < p.tile && t < p.tokens) {
-    int first = t, end = t + 1;
-    while (b < p.batch && p.cu[b + 1] <= t) ++b;
-    if (b < p.batch) { first = p.cu[b]; end = min(p.cu[b + 1], p.tokens); }
-    if (b < p.batch && first >= 0 && first <= t) {
-      const int len = p.lens[b];
-      const long long pos = (long long)len + (t - first);
-      const int off = (int)(pos % p.block);
-      if (len >= 0 && (t == first || off == 0) && pos / p.page_size < p.width) {
-        const int page = p.table[(long long)b * p.width + pos / p.page_size];
-        if (page >= 0 && page < p.num_pages) {
-          AppendBlock& g = blocks[atomicAdd(&n_blocks, 1)];
-          g.row0 = t; g.off = off; g.fresh = min(end - t, p.block - off);
-          g.page = page; g.index = (int)(pos % p.page_size) / p.block;
-        }
-      }
-    }
+  if ((int)threadIdx.x < n_listed) {
+    const int i = owner[threadIdx.x];
+    const AppendRun run(p, i);
+    const int skip = run.len & (p.block - 1);                     // tokens of the first block that are there already
+    const int r = nth[threadIdx.x] == 0 ? 0 : nth[threadIdx.x] * p.block - skip;     // the block's first new row
+    const long long pos = (long long)run.len + r;
+    AppendBlock g;
+    g.row0 = run.first + r;
+    g.off = nth[threadIdx.x] == 0 ? skip : 0;
+    g.fresh = min(run.count - r, p.block - g.off);
+    g.page = p.table[(long long)i * p.width + pos / p.page_size];
+    g.index = (int)(pos % p.page_size) / p.block;
+    if (g.page < 0 || g.page >= p.num_pages) g.fresh = 0;
+    blocks[threadIdx.x] = g;
   }
   __syncthreads();
   // ---- the tasks
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int wpt = p.warps_per_task, groups = kAppendWarps / wpt, group = warp / wpt, w = warp - group * wpt;
-  const int job0 = blockIdx.y * p.jobs_per_cta, n_jobs = min(p.jobs_per_cta, 2 * p.heads - job0);
-  const int n_tasks = n_blocks * n_jobs;
+  const int task_from = (int)max(0ll, share[0] - list0 * n_jobs);
+  const int n_tasks = (int)min((long long)n_listed * n_jobs, share[1] - list0 * n_jobs);
   const int lanes = p.head_dim >> 3, rows_at_once = 32 / lanes;      // a lane holds 8 numbers of a row
   const int my_row = lane / lanes, my_col = (lane - my_row * lanes) * 8;
   const bool active = my_row < rows_at_once;
-  struct Task {
+  struct Task {                                // (what else a task needs is looked up again: the registers are rows)
     uint4 x[kUnitRows / 2];                    // the warp's rows of the block
     float before;
-    int row0, off, fresh, which;
-    float* scale;
-    unsigned char* base;
   };
   auto load = [&](int task, Task& k) {
     if (task >= n_tasks) return;
     const AppendBlock g = blocks[task / n_jobs];
-    const int job = job0 + task % n_jobs, h = job >> 1;
-    k.which = job & 1; k.off = g.off; k.fresh = g.fresh;
-    k.scale = p.scales[k.which] + g.page * p.scale_sp[k.which] + g.index * p.scale_sb[k.which] + h * p.scale_sh[k.which];
-    k.base = (unsigned char*)p.pages[k.which] + g.page * p.page_sp[k.which] +
-             (long long)g.index * p.block * p.page_st[k.which] + h * p.page_sh[k.which];
+    const int job = task % n_jobs, which = job & 1, h = job >> 1;
     k.before = 0.f;
-    if (g.off) k.before = *k.scale;
-    const T* rows = (const T*)p.rows[k.which] + h * p.row_sh[k.which] + my_col;
+    if (g.off && g.fresh)
+      k.before = p.scales[which][g.page * p.scale_sp[which] + g.index * p.scale_sb[which] + h * p.scale_sh[which]];
+    const T* rows = (const T*)p.rows[which] + h * p.row_sh[which] + my_col;
 #pragma unroll
     for (int i = 0; i < kUnitRows / 2; ++i) {
       const int r = w * kUnitRows + i * rows_at_once + my_row - g.off;           // of the block's new rows
       k.x[i] = make_uint4(0, 0, 0, 0);
       if (active && i * rows_at_once < kUnitRows && r >= 0 && r < g.fresh)
-        k.x[i] = *reinterpret_cast<const uint4*>(rows + (long long)(g.row0 + r) * p.row_st[k.which]);
+        k.x[i] = *reinterpret_cast<const uint4*>(rows + (long long)(g.row0 + r) * p.row_st[which]);
     }
   };
   Task now, next;
-  load(group, now);
-  for (int task0 = 0, turn = 0; task0 < n_tasks; task0 += groups, turn ^= 1) {
-    const bool some = task0 + group < n_tasks;
-    load(task0 + groups + group, next);
+  load(task_from + group, now);
+  for (int task = task_from + group; task < n_tasks; task += groups, turn ^= 1) {
+    load(task + groups, next);
     unsigned top = 0;
-    if (some) {
 #pragma unroll
-      for (int i = 0; i < kUnitRows / 2; ++i) top = max_abs8<T>(top, now.x[i]);
-      top = __reduce_max_sync(0xffffffffu, larger(top));
-    }
+    for (int i = 0; i < kUnitRows / 2; ++i) top = max_abs8<T>(top, now.x[i]);
+    top = __reduce_max_sync(0xffffffffu, larger(top));
     if (wpt > 1) {                             // the warps of a task meet (two sets of places, one barrier)
       if (lane == 0) tops[turn][warp] = top;
-      __syncthreads();
+      asm volatile("bar.sync %0, %1;" :: "r"(1 + group), "r"(wpt * 32) : "memory");
       for (int i = 0; i < wpt; ++i) top = max(top, tops[turn][group * wpt + i]);
     }
-    if (some) {
+    const AppendBlock g = blocks[task / n_jobs];
+    if (g.fresh > 0) {
+      const int job = task % n_jobs, which = job & 1, h = job >> 1;
       const Scaling<T, kE4M3> sc(top, now.before);
-      const long long st = p.page_st[now.which];
-      unsigned char* const base = now.base + my_col + (w * kUnitRows + my_row) * st;
-      const int r0 = w * kUnitRows + my_row - now.off;                           // the lane's first row among the new ones
+      const long long st = p.page_st[which];
+      unsigned char* const base = (unsigned char*)p.pages[which] + g.page * p.page_sp[which] + h * p.page_sh[which] + my_col +
+                                  (g.index * p.block + w * kUnitRows + my_row) * st;
+      const int r0 = w * kUnitRows + my_row - g.off;                             // the lane's first row among the new ones
       auto store = [&](auto pow2) {
 #pragma unroll
         for (int i = 0; i < kUnitRows / 2; ++i) {
           const int r = r0 + i * rows_at_once;
-          if (active && i * rows_at_once < kUnitRows && r >= 0 && r < now.fresh)
+          if (active && i * rows_at_once < kUnitRows && r >= 0 && r < g.fresh)
             *reinterpret_cast<uint2*>(base + i * rows_at_once * st) = sc.template eight<decltype(pow2)::value>(now.x[i]);
         }
       };
       if (sc.pow2) store(std::true_type());
       else store(std::false_type());
-      if (now.off && sc.after > now.before)                                      // earlier rows to the new scale
+      if (g.off && sc.after > now.before)                                        // earlier rows to the new scale
         for (int i = 0; i * rows_at_once < kUnitRows; ++i)
           if (active && r0 + i * rows_at_once < 0) {
             uint2* at = reinterpret_cast<uint2*>(base + i * rows_at_once * st);
             *at = sc.again(*at);
           }
-      if (w == 0 && lane == 0) *now.scale = sc.after;
+      if (w == 0 && lane == 0)
+        p.scales[which][g.page * p.scale_sp[which] + g.index * p.scale_sb[which] + h * p.scale_sh[which]] = sc.after;
     }
     now = next;
+  }
+  __syncthreads();                             // (the list is read)
   }
 }
 
 template <typename T, bool kE4M3>
-cudaError_t launch_append(const AppendParams& p, cudaStream_t stream) {
+cudaError_t launch_append(const AppendParams& p, int ctas, cudaStream_t stream) {
   if (!p.cu) {
     const int jobs = 2 * p.tokens * p.heads, each = kAppendWarps * (32 / (p.head_dim / 8));
     return launch_after(append_8bit_one_kernel<T, kE4M3>, dim3((jobs + each - 1) / each), dim3(kAppendThreads), 0, stream, p);
   }
-  const dim3 grid((unsigned)((p.tokens + p.tile - 1) / p.tile),
-                  (unsigned)((2 * p.heads + p.jobs_per_cta - 1) / p.jobs_per_cta));
-  return launch_after(append_8bit_kernel<T, kE4M3>, grid, dim3(kAppendThreads), 0, stream, p);
+  return launch_after(append_8bit_kernel<T, kE4M3>, dim3(ctas), dim3(kAppendThreads), 0, stream, p);
 }
 
 }  // namespace
@@ -350,7 +401,7 @@ int kv_append_8bit(const b200attn_kv_append_8bit_args* a, cudaStream_t stream) {
   if (a->block_tokens != 16 && a->block_tokens != 32 && a->block_tokens != 64 && a->block_tokens != 128)
     return B200ATTN_ERR_MODE;
   if (a->page_size <= 0 || a->page_size % a->block_tokens != 0) return B200ATTN_ERR_MODE;
-  if (a->tokens > INT_MAX - kMaxBlockTokens || a->heads > 16384) return B200ATTN_ERR_TOO_LARGE;
+  if (a->tokens > INT_MAX - kListed || a->heads > 16384) return B200ATTN_ERR_TOO_LARGE;
   if (!a->cu_new && 2 * a->tokens * a->heads > INT_MAX - 65536) return B200ATTN_ERR_TOO_LARGE;
   const void* ptrs[4] = {a->new_k, a->new_v, a->k_pages, a->v_pages};
   for (const void* q : ptrs)
@@ -380,17 +431,15 @@ int kv_append_8bit(const b200attn_kv_append_8bit_args* a, cudaStream_t stream) {
   p.table = a->page_table; p.lens = a->seqlens; p.cu = a->cu_new;
   p.tokens = (int)a->tokens; p.batch = a->batch; p.heads = a->heads; p.head_dim = a->head_dim;
   p.page_size = a->page_size; p.block = a->block_tokens; p.num_pages = a->num_pages; p.width = a->max_pages_per_seq;
-  // Packed rows: a CTA looks after a block's worth of them, with a warp for each of a block's units, and
-  // after all heads where that still fills the chip twice over.
-  p.tile = a->block_tokens;
   p.warps_per_task = a->block_tokens / kUnitRows;
-  const int tiles = (int)((a->tokens + p.tile - 1) / p.tile), at_once = kAppendWarps / p.warps_per_task;
-  const int splits = std::max(1, std::min((2 * kCtasPerSm * di->sm_count + tiles - 1) / tiles, (2 * a->heads + at_once - 1) / at_once));
-  p.jobs_per_cta = ((2 * a->heads + splits - 1) / splits + at_once - 1) / at_once * at_once;
+  // Packed rows: as many CTAs as are resident at once, or one for each of its tasks at a time where those are fewer.
+  const long long groups = kAppendWarps / p.warps_per_task;
+  const long long tasks = 2ll * a->heads * (a->tokens / a->block_tokens + 2ll * std::min<long long>(a->batch, a->tokens));
+  const int ctas = (int)std::min<long long>((long long)kCtasPerSm * di->sm_count, (tasks + groups - 1) / groups);
   const bool e4m3 = a->cache_dtype == B200ATTN_E4M3;
-  const cudaError_t e = a->dtype == B200ATTN_F16 ? (e4m3 ? launch_append<__half, true>(p, stream) : launch_append<__half, false>(p, stream))
-                                                 : (e4m3 ? launch_append<__nv_bfloat16, true>(p, stream)
-                                                         : launch_append<__nv_bfloat16, false>(p, stream));
+  const cudaError_t e = a->dtype == B200ATTN_F16 ? (e4m3 ? launch_append<__half, true>(p, ctas, stream) : launch_append<__half, false>(p, ctas, stream))
+                                                 : (e4m3 ? launch_append<__nv_bfloat16, true>(p, ctas, stream)
+                                                         : launch_append<__nv_bfloat16, false>(p, ctas, stream));
   if (e != cudaSuccess) return B200ATTN_ERR_CUDA;
   set_launch_count(1);
   return cudaGetLastError() == cudaSuccess ? B200ATTN_OK : B200ATTN_ERR_CUDA;
