@@ -477,20 +477,21 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
         // ---- S[row, key] = Q K^T for four 8-key tiles
         float sc[4][4];
 #pragma unroll
-        for (int nt = 0; nt < 4; ++nt) {
-          sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+        for (int nt = 0; nt < 4; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
 #pragma unroll
-          for (int j = 0; j < kQJ; ++j) {
-            const uint4 k4 = lds128(ktile + piece(kWarpKeys * warp + 8 * nt + gid, kQJ * tig + j));
-            const unsigned kw[4] = {k4.x, k4.y, k4.z, k4.w};
+        for (int j = 0; j < kQJ; ++j) {
+          uint4 k4[4];
 #pragma unroll
-            for (int m = 0; m < 4; ++m) {
+          for (int nt = 0; nt < 4; ++nt) k4[nt] = lds128(ktile + piece(kWarpKeys * warp + 8 * nt + gid, kQJ * tig + j));
+#pragma unroll
+          for (int m = 0; m < 4; ++m)
+#pragma unroll
+            for (int nt = 0; nt < 4; ++nt) {     // (four sums at a time: each waits for its own last product)
               unsigned b0, b1;
-              neighbours<kE4M3>(kw[m], b0, b1);
+              neighbours<kE4M3>(m == 0 ? k4[nt].x : m == 1 ? k4[nt].y : m == 2 ? k4[nt].z : k4[nt].w, b0, b1);
               if (kNT == 2) mma_16816<__half>(sc[nt], qa[j][m][0], qa[j][m][1], qa[j][m][kNT], qa[j][m][kNT + 1], b0, b1);
               else mma_16816<__half>(sc[nt], qa[j][m][0], 0u, qa[j][m][kNT], 0u, b0, b1);
             }
-          }
         }
         // the lane's scores: keys 8 nt + 2 tig + {0, 1} of rows gid and gid + 8
         unsigned pb[kNT][4];

@@ -9,8 +9,9 @@
 //   * Where a CTA can keep the bookkeeping in shared memory (up to some ten thousand pages), every CTA of
 //     the copying grid works it out for itself from the same inputs, writes its share of the new tables
 //     and copies its share of the pages: one launch, nothing exchanged.
-//   * Beyond, one cluster of CTAs keeps the books (cluster barriers between the steps: a few hundred
-//     nanoseconds, against microseconds for a launch) and a second kernel copies from its list.
+//   * Beyond, a fork's or compaction's books are kept by one cluster of CTAs (cluster barriers between the
+//     steps: a few hundred nanoseconds, against microseconds for a launch) and a second kernel copies from
+//     its list; a hand-out, which copies nothing, spreads the tables over the chip in two launches.
 #include <limits.h>
 
 #include <algorithm>
@@ -159,10 +160,8 @@ struct GrowParams {
   int32_t* refs_out;
   int32_t* missing;
   int slots, width, pages, page_size;
-  int* header;
   int* need;       // [slots] pages a row lacks
   int* first;      // [slots] the first entry that does
-  int* rank0;      // [slots] pages that the rows before lack
   int* free_list;  // [pages]
 };
 
@@ -233,43 +232,105 @@ __device__ __forceinline__ void rank_rows(const GrowParams& p, int* rank0, int a
   if (threadIdx.x == 0) *p.missing = (int)min((long long)INT_MAX, (long long)over + max(asked - free_all, 0));
 }
 
-__global__ void __launch_bounds__(kPlanThreads, 1) grow_kernel(const GrowParams p) {
+// Large books: two launches of the whole grid.  A CTA looks at its share of the rows and lists the free ones
+// of its share of the pages; what the CTAs before it lack and have makes the ranks in the second kernel.
+struct GrowShare {
+  int free, lacks;           // pages of the CTA's share that are free; pages its rows lack
+  unsigned long long past;   // pages that its rows want past the table's width
+};
+struct GrowGridParams {
+  GrowParams book;           // (free_list: share after share, each from its first page's place on)
+  GrowShare* shares;         // [kGrowCtas]
+  int rows_each, pages_each; // shares
+};
+constexpr int kGrowCtas = 2 * 148, kGrowThreads = 256;
+
+__global__ void __launch_bounds__(kGrowThreads) grow_look_kernel(const GrowGridParams q) {
+  const GrowParams& p = q.book;
+  __shared__ unsigned long long past;
+  sm100::launch_dependents();
+  if (threadIdx.x == 0) past = 0;
+  sm100::grid_dependency_wait();
+  __syncthreads();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long row0 = (long long)blockIdx.x * q.rows_each, row1 = min((long long)p.slots, row0 + q.rows_each);
+  int lacks = 0;
+  for (long long b = row0 + warp; b < row1; b += kGrowThreads / 32) {
+    int own, first;
+    look_at_row(p, (int)b, own, first);
+    if (lane == 0) {
+      p.need[b] = own; p.first[b] = first;
+      const long long over = pages_wanted(p, (int)b) - p.width;
+      if (over > 0) atomicAdd(&past, (unsigned long long)over);
+    }
+    lacks += own;
+  }
+  const long long lo = min((long long)p.pages, (long long)blockIdx.x * q.pages_each);
+  const long long hi = min((long long)p.pages, lo + q.pages_each);
+  const int free = enumerate((int)lo, (int)hi, 0, INT_MAX,
+      [&](int i) { const int r = p.refs[i]; p.refs_out[i] = r; return r; }, [](int r) { return r <= 0; },
+      [&](int i, int rank) { p.free_list[lo + rank] = i; });
+  int all;
+  warps_before(lacks, all);
+  if (threadIdx.x == 0) q.shares[blockIdx.x] = {free, all, past};
+}
+
+__global__ void __launch_bounds__(kGrowThreads) grow_give_kernel(const GrowGridParams q) {
+  const GrowParams& p = q.book;
+  __shared__ int free_before[kGrowCtas + 1], lacks_before[kGrowCtas + 1];
   sm100::launch_dependents();
   sm100::grid_dependency_wait();
-  const int tid = cluster_rank() * kPlanThreads + threadIdx.x, threads = cluster_size() * kPlanThreads;
-  const int lane = threadIdx.x & 31, warp = tid >> 5, warps = threads >> 5;
-  int lo, hi;
-  segment(p.pages, lo, hi);
-  int free_here = 0;
-  each(lo + threadIdx.x, hi, kPlanThreads, [&](int i) { return p.refs[i]; },
-       [&](int i, int r) { p.refs_out[i] = r; free_here += r <= 0; });
-  for (int b = warp; b < p.slots; b += warps) {
-    int lacks, first;
-    look_at_row(p, b, lacks, first);
-    if (lane == 0) { p.need[b] = lacks; p.first[b] = first; }
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long row0 = (long long)blockIdx.x * q.rows_each, row1 = min((long long)p.slots, row0 + q.rows_each);
+  if (warp < 2) {            // sums over the shares before each
+    int* const to = warp == 0 ? free_before : lacks_before;
+    int run = 0;
+    for (int c0 = 0; c0 < kGrowCtas; c0 += 32) {
+      int n = c0 + lane < kGrowCtas ? (warp == 0 ? q.shares[c0 + lane].free : q.shares[c0 + lane].lacks) : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int t = __shfl_up_sync(0xffffffffu, n, o);
+        if (lane >= o) n += t;
+      }
+      if (c0 + lane < kGrowCtas) to[c0 + lane + 1] = run + n;
+      run += __shfl_sync(0xffffffffu, n, 31);
+    }
+    if (lane == 0) to[0] = 0;
   }
-  free_here = block_sum(free_here);
-  if (threadIdx.x == 0) p.header[kCountA + cluster_rank()] = free_here;
-  cluster_barrier();
-
-  int free_before, free_all, asked = 0;
-  counts_of(p.header + kCountA, free_before, free_all);
-  const auto need = [&](int b) { return __ldcg(p.need + b); };
-  each(threadIdx.x, p.slots, kPlanThreads, need, [&](int, int n) { asked += n; });
-  asked = block_sum(asked);
-  enumerate(lo, hi, free_before, asked, [&](int i) { return p.refs[i]; }, [](int r) { return r <= 0; },
-            [&](int i, int rank) { p.free_list[rank] = i; });
-  if (cluster_rank() == cluster_size() - 1) rank_rows(p, p.rank0, asked, free_all, need);
-  cluster_barrier();
-
-  for (int b0 = warp; b0 < p.slots; b0 += 32 * warps) {          // a lane looks up one of the warp's rows each
-    const long long looked = min((long long)b0 + (long long)lane * warps, (long long)p.slots - 1);
-    const int all_need = __ldcg(p.need + looked), all_first = __ldcg(p.first + looked), all_rank = __ldcg(p.rank0 + looked);
-    const int all_want = (int)min((long long)p.width, pages_wanted(p, (int)looked));
-    for (int k = 0; k < 32 && b0 + (long long)k * warps < p.slots; ++k)
-      give(p, b0 + (long long)k * warps, __shfl_sync(0xffffffffu, all_need, k), __shfl_sync(0xffffffffu, all_first, k),
-           __shfl_sync(0xffffffffu, all_want, k), __shfl_sync(0xffffffffu, all_rank, k), free_all,
-           [&](int i) { return __ldcg(p.free_list + i); });
+  __syncthreads();
+  const int free_all = free_before[kGrowCtas];
+  if (blockIdx.x == 0 && warp == 2) {
+    unsigned long long past = 0;
+    for (int c = lane; c < kGrowCtas; c += 32) past += q.shares[c].past;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) past += __shfl_xor_sync(0xffffffffu, past, o);
+    if (lane == 0)
+      *p.missing = (int)min((unsigned long long)INT_MAX, past + max(lacks_before[kGrowCtas] - free_all, 0));
+  }
+  auto page_at = [&](int rank) {
+    int lo = 0, hi = kGrowCtas;                // the share with free_before[lo] <= rank < free_before[hi = lo + 1]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (free_before[mid] <= rank) lo = mid;
+      else hi = mid;
+    }
+    return p.free_list[(long long)lo * q.pages_each + rank - free_before[lo]];
+  };
+  int rank0 = lacks_before[blockIdx.x];
+  for (long long b0 = row0; b0 < row1; b0 += 32) {               // a lane looks up one row each
+    const long long b = min(b0 + lane, row1 - 1);
+    const int own = b0 + lane < row1 ? p.need[b] : 0, first = p.first[b];
+    const int want = (int)min((long long)p.width, pages_wanted(p, (int)b));
+    int upto = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int t = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += t;
+    }
+    for (int k = warp; k < 32 && b0 + k < row1; k += kGrowThreads / 32)
+      give(p, b0 + k, __shfl_sync(0xffffffffu, own, k), __shfl_sync(0xffffffffu, first, k), __shfl_sync(0xffffffffu, want, k),
+           rank0 + __shfl_sync(0xffffffffu, upto - own, k), free_all, page_at);
+    rank0 += __shfl_sync(0xffffffffu, upto, 31);
   }
 }
 
@@ -787,7 +848,7 @@ bool grow_by_one(const b200attn_pages_grow_args* a) {
 
 size_t pages_grow_workspace_bytes(const b200attn_pages_grow_args* a) {
   if (!a || a->slots <= 0 || a->num_pages <= 0 || a->max_pages_per_seq <= 0 || grow_by_one(a)) return 0;
-  return 4 * ((size_t)kHeader + 3 * (size_t)a->slots + a->num_pages);
+  return kGrowCtas * sizeof(GrowShare) + 4 * (2 * (size_t)a->slots + a->num_pages);
 }
 
 int pages_grow(const b200attn_pages_grow_args* a, cudaStream_t stream) {
@@ -809,14 +870,17 @@ int pages_grow(const b200attn_pages_grow_args* a, cudaStream_t stream) {
     set_launch_count(1);
     return cudaGetLastError() == cudaSuccess ? B200ATTN_OK : B200ATTN_ERR_CUDA;
   }
-  p.header = (int*)a->workspace;
-  p.need = p.header + kHeader;
+  GrowGridParams q;
+  q.shares = (GrowShare*)a->workspace;
+  p.need = (int*)(q.shares + kGrowCtas);
   p.first = p.need + a->slots;
-  p.rank0 = p.first + a->slots;
-  p.free_list = p.rank0 + a->slots;
-  st = launch_plan(grow_kernel, p, 0, stream);
-  if (st != B200ATTN_OK) return st;
-  set_launch_count(1);
+  p.free_list = p.first + a->slots;
+  q.book = p;
+  q.rows_each = (int)(((long long)a->slots + kGrowCtas - 1) / kGrowCtas);
+  q.pages_each = (int)(((long long)a->num_pages + kGrowCtas - 1) / kGrowCtas);
+  for (auto kernel : {grow_look_kernel, grow_give_kernel})
+    if (launch_after(kernel, dim3(kGrowCtas), dim3(kGrowThreads), 0, stream, q) != cudaSuccess) return B200ATTN_ERR_CUDA;
+  set_launch_count(2);
   return cudaGetLastError() == cudaSuccess ? B200ATTN_OK : B200ATTN_ERR_CUDA;
 }
 
