@@ -407,7 +407,8 @@ int b200attn_kv_append(const b200attn_kv_append_args* args, b200attn_stream_t st
  *
  * k_pages / v_pages are pools [num_pages, page_size, heads_kv, head_dim] of
  * E4M3 or I8 numbers (any strides that are multiples of 16, so a pool whose
- * heads lie outside its tokens does as well), k_scales / v_scales fp32 pools
+ * heads lie outside its tokens does as well, but not 0; nor are the scales' where
+ * rows are appended), k_scales / v_scales fp32 pools
  * [num_pages, page_size / block_tokens, heads_kv]: element (page, t, h, d) stands
  * for number * scale[page][t / block_tokens][h].  block_tokens is 16, 32, 64 or
  * 128 and divides page_size.  page_table [batch, max_pages_per_seq] lists the

@@ -186,3 +186,25 @@ def test_oracle_compact_and_grow_by_hand():
     t, r, missing = orc.grow(torch.tensor([[1, -1], [-1, -1]], dtype=i32), torch.tensor([16, 0], dtype=i32),
                              torch.tensor([0, 1, 0], dtype=i32), torch.tensor([17, 20], dtype=i32), 16)
     assert t.tolist() == [[1, 0], [2, -1]] and r.tolist() == [1, 1, 1] and int(missing) == 2
+
+
+@pytest.mark.parametrize("field", ["k_stride_page", "v_stride_page", "k_stride_t", "v_stride_t", "k_stride_h", "v_stride_h",
+                                   "ks_stride_page", "vs_stride_page", "ks_stride_blk", "vs_stride_blk", "ks_stride_h",
+                                   "vs_stride_h"])
+def test_what_is_written_lies_apart(lib, field):
+    """An expanded pool or scale (a stride of 0) is refused where rows are appended, an expanded pool
+    where it is read as well."""
+    a, d = append_args(), decode_args()
+    for x, D in ((a, 64), (d, 128)):
+        for pool in "kv":
+            for f, v in (("page", 64 * 2 * D), ("t", 2 * D), ("h", D)):
+                setattr(x, f"{pool}_stride_{f}", v)
+            for f, v in (("page", 4), ("blk", 2), ("h", 1)):
+                setattr(x, f"{pool}s_stride_{f}", v)
+    d.q_stride_b = d.q_stride_t = d.o_stride_b = d.o_stride_t = 8 * 128
+    d.q_stride_h = d.o_stride_h = 128
+    setattr(a, field, 0)
+    assert lib.b200attn_kv_append_8bit(C.byref(a), None) == -6
+    if field[1] == "_":
+        setattr(d, field, 0)
+        assert lib.b200attn_paged_decode_8bit_fwd(C.byref(d), None) == -6

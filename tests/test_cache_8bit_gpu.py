@@ -591,3 +591,122 @@ def test_native_calls_equal_python_calls(monkeypatch):
     monkeypatch.setattr(ops, "_native", lambda *a: None)
     for i, (a, b) in enumerate(zip(native, results())):
         assert same_bits(a, b), i
+
+
+# ---------------------------------------------------------------------------- sizes past the kernels' own
+def test_append_more_blocks_than_a_cta_lists():
+    """One prompt of 620,000 rows beside a short one: what one call stores is, bit for bit, what calls of
+    100,000 rows store (whole blocks, so their scales are the same)."""
+    from tritonops_b200 import ops
+    D, page, block = 32, 64, 16
+    T, step = 620_000, 100_000
+    pages = -(-T // page) + 3
+    g = torch.Generator().manual_seed(57)
+    x = (torch.randn(2, T + 5, 1, D, generator=g) * torch.exp2(torch.randint(-6, 7, (2, T + 5, 1, 1), generator=g).float())).half().cuda()
+    table = torch.full((2, pages), -1, dtype=i32)
+    order = torch.randperm(pages, generator=g).to(i32)
+    table[0, :1], table[1, :pages - 2] = order[:1], order[1:pages - 1]
+    table = table.cuda()
+
+    def empty():
+        return [torch.zeros(pages, page, 1, D, dtype=E4M3, device="cuda") for _ in range(2)] + \
+               [torch.zeros(pages, page // block, 1, device="cuda") for _ in range(2)]
+
+    def lengths(*n):
+        return torch.tensor(n, dtype=i32, device="cuda")
+    whole, parts = empty(), empty()
+    ops.append_kv_8bit(*whole, x[0], x[1], table, lengths(0, 0), cu_new=lengths(0, 5, T + 5))
+    ops.append_kv_8bit(*parts, x[0, :5], x[1, :5], table, lengths(0, 0), cu_new=lengths(0, 5, 5))
+    for at in range(0, T, step):
+        n = min(step, T - at)
+        part = x[:, 5 + at:5 + at + n]
+        ops.append_kv_8bit(*parts, part[0], part[1], table, lengths(5, at), cu_new=lengths(0, 0, n))
+    for a, b in zip(whole, parts):
+        assert torch.equal(bits(a), bits(b))
+    # and a sample of the blocks are the oracle's
+    some = [0, 1, 137 * 64 // block, T // block - 1]
+    for blk in some:
+        rows = x[:, 5 + blk * block:5 + (blk + 1) * block].cpu()
+        k, v, ks, vs = [torch.zeros(1, block, 1, D).to(E4M3) for _ in range(2)] + [torch.zeros(1, 1, 1) for _ in range(2)]
+        want = orc.append(k, v, ks, vs, rows[0], rows[1], torch.zeros(1, 1, dtype=i32), torch.zeros(1, dtype=i32), [block])
+        pg, off = int(table[1, blk * block // page]), blk * block % page
+        got = [whole[0][pg:pg + 1, off:off + block], whole[1][pg:pg + 1, off:off + block],
+               whole[2][pg:pg + 1, off // block:off // block + 1], whole[3][pg:pg + 1, off // block:off // block + 1]]
+        equal_cache(got, want)
+
+
+@pytest.mark.parametrize("cdt", [E4M3, I8])
+def test_a_thousand_ragged_sequences(cdt):
+    lens = [random.Random(58 + i).choice([0, 1, 2, 15, 16, 17, 40, 129, 300]) for i in range(1100)]
+    table, pages = rows_of(59, lens, 16)
+    n = torch.tensor(lens, dtype=i32)
+    pools = cache(60, pages, 16, 16, 2, 64, cdt)
+    spoil(pools, table, n)
+    q = torch.randn(len(lens), 2, 4, 64, generator=torch.Generator().manual_seed(61)).to(torch.bfloat16)
+    check(attend(q, pools, table, n), q, pools, table, n)
+
+
+def test_drafts_do_not_see_what_comes_after_them():
+    """NaN and the largest numbers in the last drafted token reach its own query only."""
+    lens = torch.tensor([200, 64, 5], dtype=i32)
+    table, pages = rows_of(62, lens.tolist(), 16)
+    pools = cache(63, pages, 16, 16, 2, 128, E4M3)
+    q = torch.randn(3, 5, 10, 128, generator=torch.Generator().manual_seed(64)).half()
+    before = attend(q, pools, table, lens).cpu()
+    for b, n in enumerate(lens.tolist()):
+        page, at = int(table[b, (n - 1) // 16]), (n - 1) % 16
+        pools[0].view(torch.uint8)[page, at], pools[1].view(torch.uint8)[page, at] = 0x7f, 0x7f
+    after = attend(q, pools, table, lens).cpu()
+    assert torch.equal(after[:, :4], before[:, :4]) and after[:, 4].isnan().all()
+    q[:, 1] = math.nan                       # a query's NaN stays its own as well
+    odd = attend(q, pools, table, lens).cpu()
+    assert odd[:, 1].isnan().all()
+    assert torch.equal(odd[:, [0, 2, 3]], before[:, [0, 2, 3]])
+
+
+def test_calls_on_two_streams_at_once():
+    """Appends, attention and hand-outs of two caches, issued in turn on two streams."""
+    from tritonops_b200 import ops
+    lens = torch.tensor([700, 1300, 90], dtype=i32)
+    jobs = []
+    for i in (65, 66):
+        table, pages = rows_of(i, [n + 40 for n in lens.tolist()], 32)
+        g = torch.Generator().manual_seed(i)
+        pools = cache(i, pages, 32, 32, 2, 128, I8)
+        nk, nv = torch.randn(2, 3, 2, 128, generator=g).half()
+        q = torch.randn(3, 16, 128, generator=g).half()
+        refs = torch.randint(0, 2, (30000,), generator=g).to(i32)
+        want = orc.append(*pools, nk, nv, table, lens, [1] * 3)
+        jobs.append(dict(dev=[p.cuda() for p in pools], nk=nk.cuda(), nv=nv.cuda(), q=q, qd=q.cuda(), t=table.cuda(),
+                         table=table, want=want, refs=refs, refs_d=refs.cuda(), s=torch.cuda.Stream()))
+    n, one = lens.cuda(), torch.ones(3, dtype=i32, device="cuda")
+    empty = torch.full((3, 200), -1, dtype=i32)
+    ed, new = empty.cuda(), torch.tensor([1000, 50, 3000], dtype=i32)
+    newd, zero = new.cuda(), torch.zeros(3, dtype=i32, device="cuda")
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for j in jobs:
+            with torch.cuda.stream(j["s"]):
+                ops.append_kv_8bit(*j["dev"], j["nk"], j["nv"], j["t"], n)
+                j["o"] = ops.paged_decode_8bit(j["qd"], *j["dev"], j["t"], n + one)
+                j["g"] = ops.grow_pages(ed, zero, j["refs_d"], newd, page_size=16)
+    torch.cuda.synchronize()
+    for j in jobs:
+        equal_cache(j["dev"], j["want"])
+        check(j["o"], j["q"], j["want"], j["table"], lens + 1)
+        for a, b in zip(j["g"], orc.grow(empty, torch.zeros(3, dtype=i32), j["refs"], new, 16)):
+            assert torch.equal(a.cpu().flatten(), b.flatten())
+
+
+def test_expanded_pools_are_refused():
+    from tritonops_b200 import ops
+    k, v, ks, vs = [p.cuda() for p in cache(67, 4, 16, 16, 2, 64, I8)]
+    t, n = torch.zeros(1, 2, dtype=i32, device="cuda"), torch.ones(1, dtype=i32, device="cuda")
+    row = torch.zeros(1, 2, 64, dtype=torch.float16, device="cuda")
+    q = torch.zeros(1, 4, 64, dtype=torch.float16, device="cuda")
+    wide = k[:1].expand(4, -1, -1, -1)
+    for call in (lambda: ops.append_kv_8bit(wide, v, ks, vs, row, row, t, n),
+                 lambda: ops.append_kv_8bit(k, v, ks[:, :, :1].expand(-1, -1, 2), vs, row, row, t, n),
+                 lambda: ops.paged_decode_8bit(q, wide, v, ks, vs, t, n)):
+        with pytest.raises((ValueError, RuntimeError), match="STRIDE|stride"):
+            call()

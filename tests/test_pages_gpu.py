@@ -290,3 +290,16 @@ def test_no_page_left():
     same(got, want[:4])
     new = torch.full((8,), 20, dtype=i32)
     same(ops.grow_pages(table.cuda(), lens.cuda(), refs.cuda(), new.cuda(), page_size=16), orc.grow(table, lens, refs, new, 16))
+
+
+@pytest.mark.parametrize("bad", [False, True])
+@pytest.mark.parametrize("slots,width,pages,size", [(12000, 3, 20000, 16), (297, 60, 1000, 16), (2, 9000, 70001, 16)])
+def test_hand_out_of_large_books(slots, width, pages, size, bad):
+    """More rows than CTAs times a warp's look-ups, more CTAs than rows, rows past a CTA's share."""
+    from tritonops_b200 import ops
+    table, lens, refs = book(91, slots, width, pages, size, bad=bad)
+    r = random.Random(92)
+    for most in (0, 1, 3 * size, width * size * 2):
+        new = torch.tensor([r.randint(-1, most) for _ in range(slots)], dtype=i32)
+        got = ops.grow_pages(table.cuda(), lens.cuda(), refs.cuda(), new.cuda(), page_size=size)
+        same(got, orc.grow(table, lens, refs, new, size))

@@ -414,6 +414,14 @@ int kv_append_8bit(const b200attn_kv_append_8bit_args* a, cudaStream_t stream) {
                               a->v_stride_page, a->v_stride_t, a->v_stride_h};
   for (long long s : pools)
     if (s % 16 != 0) return B200ATTN_ERR_STRIDE;
+  // what is written lies apart (an axis of one may have any stride)
+  auto meets = [](long long extent, long long stride) { return extent > 1 && stride == 0; };
+  const int blocks = a->page_size / a->block_tokens;
+  if (meets(a->num_pages, a->k_stride_page) || meets(a->num_pages, a->v_stride_page) || meets(a->page_size, a->k_stride_t) ||
+      meets(a->page_size, a->v_stride_t) || meets(a->heads, a->k_stride_h) || meets(a->heads, a->v_stride_h) ||
+      meets(a->num_pages, a->ks_stride_page) || meets(a->num_pages, a->vs_stride_page) || meets(blocks, a->ks_stride_blk) ||
+      meets(blocks, a->vs_stride_blk) || meets(a->heads, a->ks_stride_h) || meets(a->heads, a->vs_stride_h))
+    return B200ATTN_ERR_STRIDE;
   const DeviceInfo* di = nullptr;
   if (int st = device_info(&di)) return st;
   set_launch_count(0);

@@ -888,6 +888,10 @@ int paged_decode_8bit_fwd(const b200attn_paged_decode_8bit_args* a, cudaStream_t
   if (const size_t need = paged_decode_8bit_workspace_bytes(a))
     if (!a->workspace || a->workspace_bytes < need) return B200ATTN_ERR_WORKSPACE;
   if ((uintptr_t)a->workspace & 15) return B200ATTN_ERR_ALIGN;
+  auto meets = [](long long extent, long long stride) { return extent > 1 && stride == 0; };
+  if (meets(a->num_pages, a->k_stride_page) || meets(a->num_pages, a->v_stride_page) || meets(a->page_size, a->k_stride_t) ||
+      meets(a->page_size, a->v_stride_t) || meets(a->heads_kv, a->k_stride_h) || meets(a->heads_kv, a->v_stride_h))
+    return B200ATTN_ERR_STRIDE;
   const DeviceInfo* di = nullptr;
   if ((st = device_info(&di)) != B200ATTN_OK) return st;
   Decode8Params p;
