@@ -13,6 +13,15 @@
 //
 // A task is one (block, head, K or V): the block's 16-row units go to a warp each, 16 bytes per lane
 // and row, stay in registers between the maximum and the rounding, and leave as 8-byte pieces.
+//
+// Bound: two bytes read and one written for each number; behind them the instructions, about five for a
+// number (56 % of the issue slots while it runs).  Measured on B200, 8 heads of 128:
+//   packed rows   6 prompts of 37 to 5000 rows, fp16 to int8 (98 MB)       23.4 us  4.2 TB/s
+//                 16 prompts of 3000 to 5000 rows, bf16 to e4m3 (411 MB)   78.7 us  5.2 TB/s, 0.81 of a copy
+//                 128 sequences of 3 to 6 rows                             12.6 us
+//     (a CTA for a run of rows, with the blocks that begin there: 27.4, 89.5 and 27.1 us: a partial second
+//     wave, and the look-ups once for every block)
+//   one row each  256 sequences 3.1 us, 64 sequences 2.4 us, replayed from a graph
 #include <limits.h>
 
 #include <algorithm>

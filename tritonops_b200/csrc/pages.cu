@@ -12,6 +12,12 @@
 //   * Beyond, a fork's or compaction's books are kept by one cluster of CTAs (cluster barriers between the
 //     steps: a few hundred nanoseconds, against microseconds for a launch) and a second kernel copies from
 //     its list; a hand-out, which copies nothing, spreads the tables over the chip in two launches.
+// Measured on B200, replayed from a graph:
+//   hand-out    8 rows of 63 entries 4.5 us (one CTA); 1024 rows of 537 entries and 327,000 pages 11.0 us,
+//               33.9 us by one cluster: 2 MB of table through eight SMs
+//   fork        one sequence into four 8.0 us; 64 into 256, 40 MB copied, 24.6 us: 8 us of books (a chain of
+//               look-ups and barriers) and the copies, whose floor is 12.3 us
+//   compaction  47 small pages 4.7 us; 0.79 GB moved 275 us, 5.8 TB/s = 0.89 of a copy (both tables included)
 #include <limits.h>
 
 #include <algorithm>
