@@ -13,10 +13,10 @@
 //     steps: a few hundred nanoseconds, against microseconds for a launch) and a second kernel copies from
 //     its list; a hand-out, which copies nothing, spreads the tables over the chip in two launches.
 // Measured on B200, replayed from a graph:
-//   hand-out    8 rows of 63 entries 4.5 us (one CTA); 1024 rows of 537 entries and 327,000 pages 11.0 us,
+//   hand-out    8 rows of 63 entries 4.1 us (one CTA); 1024 rows of 537 entries and 327,000 pages 11.0 us,
 //               33.9 us by one cluster: 2 MB of table through eight SMs
-//   fork        one sequence into four 8.0 us; 64 into 256, 40 MB copied, 24.6 us: 8 us of books (a chain of
-//               look-ups and barriers) and the copies, whose floor is 12.3 us
+//   fork        one sequence into four 7.3 us; 64 into 256, 40 MB copied, 22.4 us: 8 us of launch and books (a
+//               chain of look-ups and barriers) and the copies, whose floor is 12.3 us
 //   compaction  47 small pages 4.7 us; 0.79 GB moved 275 us, 5.8 TB/s = 0.89 of a copy (both tables included)
 #include <limits.h>
 
@@ -354,13 +354,21 @@ __global__ void __launch_bounds__(kGrowOneThreads, 1) grow_one_kernel(const Grow
   sm100::grid_dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = kGrowOneThreads / 32;
   int free_all = 0, asked = 0;
-  each(threadIdx.x, p.pages, kGrowOneThreads, [&](int i) { return p.refs[i]; },
-       [&](int i, int r) { p.refs_out[i] = r; free_all += r <= 0; });
+  // (the first counts are on their way while the rows are looked at)
+  int refs0[kAhead];
+#pragma unroll
+  for (int j = 0; j < kAhead; ++j)
+    if (threadIdx.x + j * kGrowOneThreads < p.pages) refs0[j] = p.refs[threadIdx.x + j * kGrowOneThreads];
   for (int b = warp; b < p.slots; b += warps) {
     int lacks, at;
     look_at_row(p, b, lacks, at);
     if (lane == 0) { need[b] = lacks; first[b] = at; asked += lacks; }
   }
+  auto count = [&](int i, int r) { p.refs_out[i] = r; free_all += r <= 0; };
+#pragma unroll
+  for (int j = 0; j < kAhead; ++j)
+    if (threadIdx.x + j * kGrowOneThreads < p.pages) count(threadIdx.x + j * kGrowOneThreads, refs0[j]);
+  each(threadIdx.x + kAhead * kGrowOneThreads, p.pages, kGrowOneThreads, [&](int i) { return p.refs[i]; }, count);
   free_all = block_sum(free_all);
   asked = block_sum(asked);
   rank_rows(p, rank0, asked, free_all, [&](int b) { return need[b]; });
@@ -619,14 +627,22 @@ __global__ void __launch_bounds__(kCopyThreads, 2) fork_copy_kernel(const __grid
   for (int b = tid; b < p.slots; b += kCopyThreads) { keeper[b] = INT_MAX; want[b] = -1; }
   __syncthreads();
   sm100::grid_dependency_wait();
-  each(tid, p.slots, kCopyThreads, [&](int b) { return p.lens[b]; },
-       [&](int b, int n) { lens[b] = (int)min((long long)max(n, 0), (long long)p.width * p.page_size); });
-  each(tid, p.slots, kCopyThreads, [&](int b) { return p.parents[b]; }, [&](int b, int parent) {
+  // (one trip to memory for the first of all three lists)
+  int refs0[kAhead];
+#pragma unroll
+  for (int j = 0; j < kAhead; ++j)
+    if (tid + j * kCopyThreads < p.pages) refs0[j] = p.refs[tid + j * kCopyThreads];
+  for (int b = tid; b < p.slots; b += kCopyThreads) {
+    const int n = p.lens[b], parent = p.parents[b];
+    lens[b] = (int)min((long long)max(n, 0), (long long)p.width * p.page_size);
     const bool alive = parent >= 0 && parent < p.slots;
     from[b] = !alive ? kFreed : parent == b ? kStays : parent;
     if (alive) atomicMin(&keeper[parent], parent == b ? -1 : b);
-  });
-  each(tid, p.pages, kCopyThreads, [&](int i) { return p.refs[i]; }, [&](int i, int r) { count[i] = r; });
+  }
+#pragma unroll
+  for (int j = 0; j < kAhead; ++j)
+    if (tid + j * kCopyThreads < p.pages) count[tid + j * kCopyThreads] = refs0[j];
+  each(tid + kAhead * kCopyThreads, p.pages, kCopyThreads, [&](int i) { return p.refs[i]; }, [&](int i, int r) { count[i] = r; });
   __syncthreads();
   auto length = [&](int b) -> int {      // of the sequence that slot b becomes
     const int parent = from[b] == kStays ? b : from[b];
@@ -645,7 +661,7 @@ __global__ void __launch_bounds__(kCopyThreads, 2) fork_copy_kernel(const __grid
     const int parent = from[b];
     return parent == kFreed ? -1 : p.table[(long long)(parent == kStays ? b : parent) * p.width + i];
   };
-  constexpr int kRows = kAhead / 2;
+  constexpr int kRows = kAhead;
   for (int b0 = warp * kRows; b0 < p.slots; b0 += warps * kRows)
     for (int i = lane; i < p.width; i += 32) {
       int gone[kRows], taken[kRows];
