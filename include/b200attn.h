@@ -470,7 +470,7 @@ typedef struct {
   int32_t num_pages, max_pages_per_seq;
   const int32_t* page_table;   /* int32 [batch, max_pages_per_seq] */
   const int32_t* seqlens;      /* int32 [batch]: tokens each sequence holds before the call */
-  const int32_t* cu_new;       /* int32 [batch+1]: the new rows of each sequence; NULL: one each */
+  const int32_t* cu_new;       /* int32 [batch+1], ascending: the new rows of each sequence; NULL: one each */
   int64_t nk_stride_t, nk_stride_h;
   int64_t nv_stride_t, nv_stride_h;
   int64_t k_stride_page, k_stride_t, k_stride_h;

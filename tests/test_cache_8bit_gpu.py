@@ -710,3 +710,27 @@ def test_expanded_pools_are_refused():
                  lambda: ops.paged_decode_8bit(q, wide, v, ks, vs, t, n)):
         with pytest.raises((ValueError, RuntimeError), match="STRIDE|stride"):
             call()
+
+
+@pytest.mark.parametrize("chunk", [2 ** 31 - 128, 2 ** 30])
+def test_one_chunk_of_any_size(chunk):
+    lens = torch.tensor([700, 3], dtype=i32)
+    table, pages = rows_of(68, lens.tolist(), 64)
+    pools = cache(69, pages, 64, 64, 1, 64, E4M3)
+    q = torch.randn(2, 4, 64, generator=torch.Generator().manual_seed(70)).half()
+    check(attend(q, pools, table, lens, chunk=chunk), q, pools, table, lens)
+
+
+def test_counts_that_do_not_ascend_store_nothing_elsewhere():
+    """cu_new that names rows again and again: pages of other rows of the table stay as they are."""
+    D, heads, page, block = 32, 1, 16, 16
+    S, T = 64, 4096
+    pages = S + 4
+    pools = cache(71, pages, page, block, heads, D, I8)
+    table = torch.full((S, 1), -1, dtype=i32)
+    table[:S // 2, 0] = torch.arange(S // 2, dtype=i32)
+    cu = torch.tensor([0, T] * (S // 2) + [0], dtype=i32)
+    nk, nv = torch.randn(2, T, heads, D, generator=torch.Generator().manual_seed(72)).half()
+    dev = append(pools, nk, nv, table, torch.zeros(S, dtype=i32), cu)
+    for a, b in zip(dev, pools):
+        assert same_bits(a[S // 2:], b[S // 2:])

@@ -277,7 +277,7 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
       const int len = min(max(head.len, 0), p.max_len);
       const int n_vis = visible(p, len, p.by_group.quotient(min(row0 + kRowsTile, p.rows) - 1));
       const int c_begin = min(head.chunk_id * p.chunk, n_vis);
-      const int c_end = min(n_vis, c_begin + p.chunk);
+      const int c_end = c_begin + min(n_vis - c_begin, p.chunk);
       const int n_stages = (c_end - c_begin + kStageKeys - 1) / kStageKeys;
       const int ask_at = max(n_stages - 8, 0), fetch_at = max(n_stages - 5, 1), scales_at = max(n_stages - 2, 2);
       // lane i looks after unit i of four stages
@@ -704,7 +704,7 @@ __global__ void __launch_bounds__(32 * kCombineWarps) decode_8bit_combine_kernel
   const int query = p.by_group.quotient(row), head = p.by_group.remainder(row);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n = visible(p, length_of(p, b), query);
-  const int nchunk = (n + p.chunk - 1) / p.chunk;
+  const int nchunk = n > 0 ? (n - 1) / p.chunk + 1 : 0;
   const long long row0 = ((long long)(b * p.heads_kv + hk) * p.rows + row) * p.max_chunks;
   const float* lse = p.part_lse + row0;
   float M = -INFINITY;
