@@ -45,6 +45,13 @@ constexpr int kUnits = kStageKeys / kUnitKeys;
 constexpr int kRowsTile = 16;      // query rows (query x head of the group) of a work item
 constexpr float kPUp = 10.f;       // P is 2^kPUp times the weight
 
+// CTAs per SM: 192 KB are in flight either way.  With heads of up to 64 and up to 8 rows the copies' issue and the
+// warps' chains bound, of which three CTAs have more under way: 64 sequences of 4096 keys, D = 64, 107 us -> 81 in
+// pages of 16 keys, 67 -> 60 in pages of 64; two of 60000, 62 -> 49 and 43 -> 40; 128 of 100 to 2000, 68 -> 66 and
+// 44 -> 47.  The registers that three leave are few for 16 rows (D = 64: 20 rows, 24 sequences of 300 to 6000, 81 us ->
+// 92; D = 128: 32 of 4096, 87 -> 118), and with D = 128 two stages are few for the memory (92 -> 104 with one row).
+__host__ __device__ constexpr int ctas_per_sm(int head_dim, int rows) { return head_dim <= 64 && rows <= 8 ? 3 : 2; }
+
 // n / d for 0 <= n < 2^31 by a multiplication (a division by a run-time number takes the producer
 // warp longer than the copy it prepares)
 struct Divisor {
@@ -96,11 +103,11 @@ struct Decode8Item {
 constexpr int kConsumers = kStageKeys / kWarpKeys;   // warps
 constexpr int kDecode8Threads = 32 * kConsumers + 32;
 
-template <int DP>
+template <int DP, int kRows>
 struct Decode8Smem {
   static constexpr int kTileBytes = kStageKeys * DP;       // K or V of one stage
   static constexpr int kStageBytes = 2 * kTileBytes;
-  static constexpr int kStages = DP == 128 ? 3 : 6;
+  static constexpr int kStages = 192 * 1024 / ctas_per_sm(DP, kRows) / kStageBytes;
   static constexpr int kQ = kStages * kStageBytes;         // the item's 16 query rows, fp16
   static constexpr int kQPitch = DP * 2 + 16;              // bytes
   static constexpr int kMl = kQ + kRowsTile * kQPitch;     // row max and sum, [2][warps][16]
@@ -114,7 +121,7 @@ struct Decode8Smem {
   static constexpr int kAlloc = kBytes + 1024;
   static_assert(kScales % 8 == 0 && kNext % 16 == 0 && kBarOffset % 8 == 0, "aligned");
   static_assert(kStageBytes == kConsumers * 16 * DP * 4, "the warps' sums of 16 rows fold in the buffer of a stage");
-  static_assert(2 * (kAlloc + 1024) <= 228 * 1024, "two CTAs per SM");
+  static_assert(ctas_per_sm(DP, kRows) * (kAlloc + 1024) <= 228 * 1024, "resident together");
 };
 
 __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, unsigned& r0, unsigned& r1, unsigned& r2, unsigned& r3) {
@@ -177,10 +184,10 @@ __device__ __forceinline__ void alternates(unsigned w, unsigned& even, unsigned&
 
 // T: the type of q and o.  kRows: 8 or 16 query rows are in use.
 template <typename T, bool kE4M3, int DP, int kRows>
-__global__ void __launch_bounds__(kDecode8Threads, 2)
+__global__ void __launch_bounds__(kDecode8Threads, ctas_per_sm(DP, kRows))
 decode_8bit_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                    const Decode8Params p) {
-  using L = Decode8Smem<DP>;
+  using L = Decode8Smem<DP, kRows>;
   using namespace sm100;
   constexpr int kChunks16 = DP / 16;      // 16-byte pieces of a row
   constexpr int kQJ = DP / 64;            // pieces of a K row a lane takes
@@ -220,8 +227,8 @@ decode_8bit_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
   };
   if (warp == kConsumers) {
     // ================================================================ producer
-    // Everything small that a copy needs is asked for long before it: behind a full ring (two CTAs'
-    // 192 KB per SM) a load takes as long as those bytes take to arrive, 3 to 4 us.  So nothing below
+    // Everything small that a copy needs is asked for long before it: behind full rings (192 KB
+    // per SM) a load takes as long as those bytes take to arrive, 3 to 4 us.  So nothing below
     // computes with a loaded value until stages later: a batch of units' page-table entries are asked
     // for two batches ahead and its scales one, the next item while this one's last eight stages leave.
     constexpr int kVec = DP / 8;        // 16-byte pieces of a query row
@@ -788,15 +795,15 @@ long long rows_of(const b200attn_paged_decode_8bit_args* a) {
 // 1024-8192 118.7 in 2048, 125 in 1024, 132 in one; 16 of 1024-8192 47.3 in 2048, 44.0 in 1536, 49.6 in
 // 4096; 12 of 4096 26.0 in 1536, 28.6 in 2048; 8 of 2048 13.5 in 512, 15.3 in 768; four of 90001-131072
 // 156.6 in 2048, 151 in 4096, 182 in 8192; one of 8192 10.9 in 256, 13.4 in 128.
-constexpr long long kSlots = 2 * 148;
 int chunk_of(const b200attn_paged_decode_8bit_args* a) {
   if (a->chunk_tokens > 0) return a->chunk_tokens;
   const long long units = a->batch * (long long)a->heads_kv * ((rows_of(a) + kRowsTile - 1) / kRowsTile);
   const long long stages = std::max<long long>((max_visible(a) + kStageKeys - 1) / kStageKeys, 1);
+  const long long slots = 148 * ctas_per_sm(a->head_dim, (int)std::min<long long>(rows_of(a), kRowsTile));
   long long best = 0, least = 0;
   auto consider = [&](long long per) {
     const long long n = (stages + per - 1) / per;
-    const long long cost = 2 * ((units * n + kSlots - 1) / kSlots) * (per + 4) + per + (n > 1 ? 8 : 0);
+    const long long cost = 2 * ((units * n + slots - 1) / slots) * (per + 4) + per + (n > 1 ? 8 : 0);
     if (!best || cost < least) { best = per; least = cost; }
   };
   const int sizes[10] = {1, 2, 3, 4, 6, 8, 12, 16, 32, 64};
@@ -843,7 +850,7 @@ bool pool_map(CUtensorMap* m, const void* base, const b200attn_paged_decode_8bit
 
 template <typename T, bool kE4M3, int DP, int kRows>
 int launch_split(const b200attn_paged_decode_8bit_args* a, const Decode8Params& p, dim3 grid, cudaStream_t stream) {
-  using L = Decode8Smem<DP>;
+  using L = Decode8Smem<DP, kRows>;
   auto kernel = decode_8bit_kernel<T, kE4M3, DP, kRows>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAlloc) != cudaSuccess)
     return B200ATTN_ERR_CUDA;
@@ -916,7 +923,7 @@ int paged_decode_8bit_fwd(const b200attn_paged_decode_8bit_args* a, cudaStream_t
   p.box_keys = std::min(a->page_size & -a->page_size, kStageKeys);
   p.chunk = chunk_of(a); p.max_chunks = (int)chunks;
   p.direct_o = chunks == 1;
-  p.take_over = a->heads_kv * tiles * a->batch * chunks > 2LL * di->sm_count;
+  p.take_over = a->heads_kv * tiles * a->batch * chunks > (long long)ctas_per_sm(a->head_dim, p.rows) * di->sm_count;
   p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
   p.part_o = (float*)a->workspace;
   p.part_lse = p.part_o + (size_t)a->batch * a->queries * a->heads_q * chunks * a->head_dim;
