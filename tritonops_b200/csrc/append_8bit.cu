@@ -65,7 +65,7 @@ struct AppendBlock {
 struct AppendRun {
   int first, count, len, blocks;
   __device__ __forceinline__ AppendRun(const AppendParams& p, int i) : first(0), count(0), len(0), blocks(0) {
-    if (i >= p.batch) return;
+    if (i < 0 || i >= p.batch) return;
     first = p.cu[i];
     const int end = min(p.cu[i + 1], p.tokens);
     len = p.lens[i];
@@ -287,8 +287,8 @@ __global__ void __launch_bounds__(kAppendThreads, kCtasPerSm) append_8bit_kernel
     const AppendRun run(p, i0 + threadIdx.x);
     long long all;
     const long long mine = at + sum_before(run.blocks, sums, all);
-    const int end = (int)min((long long)n_listed, mine + run.blocks);
-    for (int j = (int)max(0ll, mine); j < end; ++j) {
+    const int end = (int)max(0ll, min((long long)n_listed, mine + run.blocks));
+    for (int j = (int)max(0ll, min((long long)n_listed, mine)); j < end; ++j) {
       owner[j] = i0 + threadIdx.x;
       nth[j] = (int)(j - mine);
     }
@@ -298,16 +298,19 @@ __global__ void __launch_bounds__(kAppendThreads, kCtasPerSm) append_8bit_kernel
   if ((int)threadIdx.x < n_listed) {
     const int i = owner[threadIdx.x];
     const AppendRun run(p, i);
-    const int skip = run.len & (p.block - 1);                     // tokens of the first block that are there already
-    const int r = nth[threadIdx.x] == 0 ? 0 : nth[threadIdx.x] * p.block - skip;     // the block's first new row
-    const long long pos = (long long)run.len + r;
-    AppendBlock g;
-    g.row0 = run.first + r;
-    g.off = nth[threadIdx.x] == 0 ? skip : 0;
-    g.fresh = min(run.count - r, p.block - g.off);
-    g.page = p.table[(long long)i * p.width + pos / p.page_size];
-    g.index = (int)(pos % p.page_size) / p.block;
-    if (g.page < 0 || g.page >= p.num_pages) g.fresh = 0;
+    AppendBlock g = {0, 0, 0, 0, 0};
+    const int at_block = nth[threadIdx.x];
+    if (at_block >= 0 && at_block < run.blocks) {                 // (always, unless someone writes the lengths meanwhile)
+      const int skip = run.len & (p.block - 1);                   // tokens of the first block that are there already
+      const int r = at_block == 0 ? 0 : at_block * p.block - skip;     // the block's first new row
+      const long long pos = (long long)run.len + r;
+      const int page = p.table[(long long)i * p.width + pos / p.page_size];
+      g.row0 = run.first + r;
+      g.off = at_block == 0 ? skip : 0;
+      if (page >= 0 && page < p.num_pages) g.fresh = min(run.count - r, p.block - g.off);
+      g.page = page;
+      g.index = (int)(pos % p.page_size) / p.block;
+    }
     blocks[threadIdx.x] = g;
   }
   __syncthreads();
