@@ -790,11 +790,17 @@ int check_pools(const b200attn_page_pool* pools, int n) {
   return B200ATTN_OK;
 }
 
+// Raises the kernel's limit where it has to be.  48 KB are granted without asking, of which the kernel's own
+// __shared__ variables (144 bytes at most in this file) take their part.
+template <typename P>
+bool allow(void (*kernel)(P), size_t smem) {
+  return smem <= 47 * 1024 ||
+         cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) == cudaSuccess;
+}
+
 template <typename P>
 int launch_plan(void (*kernel)(P), const P& p, size_t smem, cudaStream_t stream) {
-  if (smem > 48 * 1024 &&
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-    return B200ATTN_ERR_CUDA;
+  if (!allow(kernel, smem)) return B200ATTN_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(kPlanCtas);
   cfg.blockDim = dim3(kPlanThreads);
@@ -842,9 +848,7 @@ int launch_copies(const b200attn_page_pool* pools, int n_pools, const int* count
 template <typename P, typename B>
 int launch_both(void (*kernel)(P), const B& book, size_t smem, const b200attn_page_pool* pools, int n_pools, int sm_count,
                 cudaStream_t stream, int& launches) {
-  if (smem > 48 * 1024 &&
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-    return B200ATTN_ERR_CUDA;
+  if (!allow(kernel, smem)) return B200ATTN_ERR_CUDA;
   for (int at = 0; at == 0 || at < n_pools; at += kCopyPools) {
     P p;
     p.book = book;
@@ -888,6 +892,7 @@ int pages_grow(const b200attn_pages_grow_args* a, cudaStream_t stream) {
   p.slots = a->slots; p.width = a->max_pages_per_seq; p.pages = a->num_pages; p.page_size = a->page_size;
   if (grow_by_one(a)) {
     const size_t smem = 4 * (3 * (size_t)a->slots + a->num_pages);
+    if (!allow(grow_one_kernel, smem)) return B200ATTN_ERR_CUDA;
     if (launch_after(grow_one_kernel, dim3(1), dim3(kGrowOneThreads), smem, stream, p) != cudaSuccess) return B200ATTN_ERR_CUDA;
     set_launch_count(1);
     return cudaGetLastError() == cudaSuccess ? B200ATTN_OK : B200ATTN_ERR_CUDA;
