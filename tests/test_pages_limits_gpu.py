@@ -1,8 +1,9 @@
 """Page operators at the sizes where a kernel's shared memory passes what is granted without asking
-(48 KB, the kernel's own variables included)."""
+(48 KB, the kernel's own variables included), and from several host threads at once."""
 import os
 import subprocess
 import sys
+import threading
 
 import pytest
 import torch
@@ -88,3 +89,47 @@ def test_sizes_at_the_granted_shared_memory():
     code = f"import sys; sys.path[:0] = [{os.path.dirname(HERE)!r}, {HERE!r}]; import test_pages_limits_gpu as t; t.every_size()"
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=600)
     assert r.returncode == 0, r.stderr[-4000:]
+
+
+def in_threads(*calls):
+    """Each of `calls` over and over on four threads with a stream each; what they raised."""
+    calls = calls * 4
+    raised, ready = [], threading.Barrier(len(calls), timeout=60)
+    torch.cuda.synchronize()
+
+    def loop(call):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            ready.wait()
+            try:
+                for _ in range(10000):
+                    call()
+            except (RuntimeError, ValueError) as e:
+                raised.append(str(e))
+
+    threads = [threading.Thread(target=loop, args=(c,)) for c in calls]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    return raised
+
+
+def test_small_and_large_books_from_several_threads():
+    """No call lowers the limit that another thread's launch relies on."""
+    from tritonops_b200 import ops
+
+    def forks(slots, pages):
+        table, lens, refs = (t.cuda() for t in book(slots, 4, pages))
+        par = torch.arange(slots, dtype=i32, device="cuda") // 4 * 4
+        return lambda: ops.fork_pages([], table, lens, refs, par, page_size=16)
+
+    def compactions(pages):
+        table, _, refs = (t.cuda() for t in book(16, 40, pages))
+        return lambda: ops.compact_pages([], table, refs)
+
+    bad = []
+    bad += in_threads(forks(64, 12400), forks(64, 28000))
+    bad += in_threads(compactions(6400), compactions(14000))
+    bad += in_threads(forks(12400, 12400), forks(32768, 32768))
+    assert not bad

@@ -790,17 +790,18 @@ int check_pools(const b200attn_page_pool* pools, int n) {
   return B200ATTN_OK;
 }
 
-// Raises the kernel's limit where it has to be.  48 KB are granted without asking, of which the kernel's own
-// __shared__ variables (144 bytes at most in this file) take their part.
+// Raises the kernel's limit where `smem` needs it.  48 KB are granted without asking, of which the kernel's own
+// __shared__ variables (144 bytes at most in this file) take their part.  The limit is the process's, so it is always
+// set to the same number, the most that any call of the kernel asks for: another thread may be about to launch.
 template <typename P>
-bool allow(void (*kernel)(P), size_t smem) {
+bool allow(void (*kernel)(P), size_t smem, size_t most) {
   return smem <= 47 * 1024 ||
-         cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) == cudaSuccess;
+         cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most) == cudaSuccess;
 }
 
 template <typename P>
 int launch_plan(void (*kernel)(P), const P& p, size_t smem, cudaStream_t stream) {
-  if (!allow(kernel, smem)) return B200ATTN_ERR_CUDA;
+  if (!allow(kernel, smem, 4 * kMaxSlots)) return B200ATTN_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(kPlanCtas);
   cfg.blockDim = dim3(kPlanThreads);
@@ -844,11 +845,14 @@ int launch_copies(const b200attn_page_pool* pools, int n_pools, const int* count
   return B200ATTN_OK;
 }
 
+// Shared memory with which two CTAs fit an SM.
+constexpr size_t kBothSmem = 112 * 1024;
+
 // Books and copies in one kernel, again for every kCopyPools pools (once without any).
 template <typename P, typename B>
 int launch_both(void (*kernel)(P), const B& book, size_t smem, const b200attn_page_pool* pools, int n_pools, int sm_count,
                 cudaStream_t stream, int& launches) {
-  if (!allow(kernel, smem)) return B200ATTN_ERR_CUDA;
+  if (!allow(kernel, smem, kBothSmem)) return B200ATTN_ERR_CUDA;
   for (int at = 0; at == 0 || at < n_pools; at += kCopyPools) {
     P p;
     p.book = book;
@@ -859,8 +863,6 @@ int launch_both(void (*kernel)(P), const B& book, size_t smem, const b200attn_pa
   }
   return B200ATTN_OK;
 }
-// Shared memory with which two CTAs fit an SM.
-constexpr size_t kBothSmem = 112 * 1024;
 size_t fork_smem(long long pages, long long slots) { return 4 * (size_t)(pages + 8 * slots); }
 size_t compact_smem(long long pages) { return 4 * (size_t)(pages + 2 * (pages / 2 + 1)); }
 
@@ -892,7 +894,7 @@ int pages_grow(const b200attn_pages_grow_args* a, cudaStream_t stream) {
   p.slots = a->slots; p.width = a->max_pages_per_seq; p.pages = a->num_pages; p.page_size = a->page_size;
   if (grow_by_one(a)) {
     const size_t smem = 4 * (3 * (size_t)a->slots + a->num_pages);
-    if (!allow(grow_one_kernel, smem)) return B200ATTN_ERR_CUDA;
+    if (!allow(grow_one_kernel, smem, 4 * kGrowOneInts)) return B200ATTN_ERR_CUDA;
     if (launch_after(grow_one_kernel, dim3(1), dim3(kGrowOneThreads), smem, stream, p) != cudaSuccess) return B200ATTN_ERR_CUDA;
     set_launch_count(1);
     return cudaGetLastError() == cudaSuccess ? B200ATTN_OK : B200ATTN_ERR_CUDA;
