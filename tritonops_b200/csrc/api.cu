@@ -38,6 +38,13 @@ int device_info(const DeviceInfo** info) {
 
 using namespace b200attn;
 
+// A CUDA error that a call has answered with is taken from the runtime as well: left there, the next call's
+// look at it after its launches would report it again, for work that it did launch.
+static int answered(int status) {
+  if (status == B200ATTN_ERR_CUDA) cudaGetLastError();
+  return status;
+}
+
 extern "C" {
 
 int b200attn_abi_version(void) { return B200ATTN_ABI_VERSION; }
@@ -69,17 +76,17 @@ size_t b200attn_decode_workspace_bytes(const b200attn_decode_args* args) {
 
 int b200attn_decode_fwd(const b200attn_decode_args* args, b200attn_stream_t stream) {
   set_launch_count(0);
-  return decode_fwd(args, false, nullptr, 0, (cudaStream_t)stream);
+  return answered(decode_fwd(args, false, nullptr, 0, (cudaStream_t)stream));
 }
 
 int b200attn_sparse_decode_fwd(const b200attn_decode_args* args, b200attn_stream_t stream) {
   set_launch_count(0);
-  return decode_fwd(args, true, nullptr, 0, (cudaStream_t)stream);
+  return answered(decode_fwd(args, true, nullptr, 0, (cudaStream_t)stream));
 }
 
 int b200attn_decode_fwd_noalloc(const b200attn_decode_args* args, b200attn_stream_t stream) {
   set_launch_count(0);
-  return decode_fwd_noalloc(args, (cudaStream_t)stream);
+  return answered(decode_fwd_noalloc(args, (cudaStream_t)stream));
 }
 
 size_t b200attn_prefill_bwd_workspace_bytes(const b200attn_prefill_bwd_args* args) {
@@ -88,17 +95,17 @@ size_t b200attn_prefill_bwd_workspace_bytes(const b200attn_prefill_bwd_args* arg
 
 int b200attn_prefill_bwd(const b200attn_prefill_bwd_args* args, b200attn_stream_t stream) {
   set_launch_count(0);
-  return prefill_bwd(args, (cudaStream_t)stream);
+  return answered(prefill_bwd(args, (cudaStream_t)stream));
 }
 
 int b200attn_kv_pack_to_cache(const b200attn_kv_pack_args* args, b200attn_stream_t stream) {
   set_launch_count(0);
-  return kv_pack_to_cache(args, (cudaStream_t)stream);
+  return answered(kv_pack_to_cache(args, (cudaStream_t)stream));
 }
 
 int b200attn_kv_append(const b200attn_kv_append_args* args, b200attn_stream_t stream) {
   set_launch_count(0);
-  return kv_append(args, (cudaStream_t)stream);
+  return answered(kv_append(args, (cudaStream_t)stream));
 }
 
 size_t b200attn_paged_decode_workspace_bytes(const b200attn_paged_decode_args* args) {
@@ -107,7 +114,7 @@ size_t b200attn_paged_decode_workspace_bytes(const b200attn_paged_decode_args* a
 
 int b200attn_paged_decode_fwd(const b200attn_paged_decode_args* args, b200attn_stream_t stream) {
   set_launch_count(0);
-  return paged_decode_fwd(args, (cudaStream_t)stream);
+  return answered(paged_decode_fwd(args, (cudaStream_t)stream));
 }
 
 int32_t b200attn_window_blocks_prefill_max_nnz(int32_t block_size, int32_t window_local, int32_t window_global,
@@ -117,17 +124,17 @@ int32_t b200attn_window_blocks_prefill_max_nnz(int32_t block_size, int32_t windo
 
 int b200attn_window_blocks_prefill(const b200attn_window_blocks_prefill_args* args, b200attn_stream_t stream) {
   set_launch_count(0);
-  return window_blocks_prefill(args, (cudaStream_t)stream);
+  return answered(window_blocks_prefill(args, (cudaStream_t)stream));
 }
 
 int b200attn_window_blocks_decode(const b200attn_window_blocks_decode_args* args, b200attn_stream_t stream) {
   set_launch_count(0);
-  return window_blocks_decode(args, (cudaStream_t)stream);
+  return answered(window_blocks_decode(args, (cudaStream_t)stream));
 }
 
 int b200attn_topk_blocks(const b200attn_topk_blocks_args* args, b200attn_stream_t stream) {
   set_launch_count(0);
-  return topk_blocks(args, (cudaStream_t)stream);
+  return answered(topk_blocks(args, (cudaStream_t)stream));
 }
 
 size_t b200attn_paged_decode_8bit_workspace_bytes(const b200attn_paged_decode_8bit_args* args) {
@@ -136,12 +143,12 @@ size_t b200attn_paged_decode_8bit_workspace_bytes(const b200attn_paged_decode_8b
 
 int b200attn_paged_decode_8bit_fwd(const b200attn_paged_decode_8bit_args* args, b200attn_stream_t stream) {
   set_launch_count(0);
-  return paged_decode_8bit_fwd(args, (cudaStream_t)stream);
+  return answered(paged_decode_8bit_fwd(args, (cudaStream_t)stream));
 }
 
 int b200attn_kv_append_8bit(const b200attn_kv_append_8bit_args* args, b200attn_stream_t stream) {
   set_launch_count(0);
-  return kv_append_8bit(args, (cudaStream_t)stream);
+  return answered(kv_append_8bit(args, (cudaStream_t)stream));
 }
 
 size_t b200attn_pages_grow_workspace_bytes(const b200attn_pages_grow_args* args) {
@@ -150,7 +157,7 @@ size_t b200attn_pages_grow_workspace_bytes(const b200attn_pages_grow_args* args)
 
 int b200attn_pages_grow(const b200attn_pages_grow_args* args, b200attn_stream_t stream) {
   set_launch_count(0);
-  return pages_grow(args, (cudaStream_t)stream);
+  return answered(pages_grow(args, (cudaStream_t)stream));
 }
 
 size_t b200attn_pages_fork_workspace_bytes(const b200attn_pages_fork_args* args) {
@@ -159,7 +166,7 @@ size_t b200attn_pages_fork_workspace_bytes(const b200attn_pages_fork_args* args)
 
 int b200attn_pages_fork(const b200attn_pages_fork_args* args, b200attn_stream_t stream) {
   set_launch_count(0);
-  return pages_fork(args, (cudaStream_t)stream);
+  return answered(pages_fork(args, (cudaStream_t)stream));
 }
 
 size_t b200attn_pages_compact_workspace_bytes(const b200attn_pages_compact_args* args) {
@@ -168,12 +175,12 @@ size_t b200attn_pages_compact_workspace_bytes(const b200attn_pages_compact_args*
 
 int b200attn_pages_compact(const b200attn_pages_compact_args* args, b200attn_stream_t stream) {
   set_launch_count(0);
-  return pages_compact(args, (cudaStream_t)stream);
+  return answered(pages_compact(args, (cudaStream_t)stream));
 }
 
 int b200attn_rmsnorm_fwd(const b200attn_rmsnorm_fwd_args* args, b200attn_stream_t stream) {
   set_launch_count(0);
-  return rmsnorm_fwd(args, (cudaStream_t)stream);
+  return answered(rmsnorm_fwd(args, (cudaStream_t)stream));
 }
 
 size_t b200attn_rmsnorm_bwd_workspace_bytes(const b200attn_rmsnorm_bwd_args* args) {
@@ -182,32 +189,32 @@ size_t b200attn_rmsnorm_bwd_workspace_bytes(const b200attn_rmsnorm_bwd_args* arg
 
 int b200attn_rmsnorm_bwd(const b200attn_rmsnorm_bwd_args* args, b200attn_stream_t stream) {
   set_launch_count(0);
-  return rmsnorm_bwd(args, (cudaStream_t)stream);
+  return answered(rmsnorm_bwd(args, (cudaStream_t)stream));
 }
 
 int b200attn_selftest_bounded_wait(int32_t* status_word, int64_t budget_cycles, int64_t* waited_cycles,
                                    b200attn_stream_t stream) {
   set_launch_count(0);
-  return selftest_bounded_wait(status_word, (long long)budget_cycles, (long long*)waited_cycles, (cudaStream_t)stream);
+  return answered(selftest_bounded_wait(status_word, (long long)budget_cycles, (long long*)waited_cycles, (cudaStream_t)stream));
 }
 
 size_t b200attn_prefill_workspace_bytes(const b200attn_prefill_args*) { return 0; }
 
 int b200attn_prefill_fwd(const b200attn_prefill_args* args, b200attn_stream_t stream) {
   set_launch_count(0);
-  return prefill_fwd(args, false, (cudaStream_t)stream);
+  return answered(prefill_fwd(args, false, (cudaStream_t)stream));
 }
 
 int b200attn_prefill_fwd_rows(const b200attn_prefill_args* args, int32_t row_begin, int32_t row_end,
                               b200attn_stream_t stream) {
   set_launch_count(0);
   if (row_begin == 0 && row_end == 0x7fffffff) row_end -= 1;   // (that pair means "all rows" internally)
-  return prefill_fwd(args, false, (cudaStream_t)stream, row_begin, row_end);
+  return answered(prefill_fwd(args, false, (cudaStream_t)stream, row_begin, row_end));
 }
 
 int b200attn_sparse_prefill_fwd(const b200attn_prefill_args* args, b200attn_stream_t stream) {
   set_launch_count(0);
-  return prefill_fwd(args, true, (cudaStream_t)stream);
+  return answered(prefill_fwd(args, true, (cudaStream_t)stream));
 }
 
 }  // extern "C"
