@@ -166,6 +166,12 @@ struct StreamSmem {
   static constexpr int kWeights = kRingBytes;                                  // fp32 [D]
   __host__ __device__ static int bars(int D) { return kWeights + ((D * 4 + 127) & ~127); }
   static int bytes(int D) { return bars(D) + 2 * kMaxSlots * 8 + 16 + 128; }   // + slack to align the base
+  // A kernel's limit is the process's and widths share the kernel: it is set to the widest row's bytes whatever the
+  // call's own, which another thread's call could otherwise lower before this one launches.
+  template <typename K>
+  static bool allow(K kernel, int widest) {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes(widest)) == cudaSuccess;
+  }
 };
 
 // ---- forward: a row per consumer warp: sum of squares, then y = x r w written over the row in
@@ -670,8 +676,7 @@ int launch_fwd(const b200attn_rmsnorm_fwd_args* a, cudaStream_t stream) {
     const int grid = (int)(a->rows < di->sm_count ? a->rows : di->sm_count);
     auto kern = rmsnorm_fwd_stream_kernel<XT, WT>;
     const int smem = StreamSmem::bytes(a->dim);
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-      return B200ATTN_ERR_CUDA;
+    if (!StreamSmem::allow(kern, kRingBytes / kFwdStreamConsumers / (int)sizeof(XT))) return B200ATTN_ERR_CUDA;
     if (launch_after(kern, dim3(grid), dim3(kFwdStreamThreads), smem, stream, (const XT*)a->x, (const WT*)a->weight,
                      (XT*)a->y, a->rstd, a->rows, a->dim, a->x_stride_row, a->y_stride_row, a->eps, slot,
                      n_slots) != cudaSuccess)
@@ -723,8 +728,7 @@ int launch_bwd_rms(const b200attn_rmsnorm_bwd_args* a, cudaStream_t stream) {
 #define B200ATTN_RMS_BWD_STREAM(CH)                                                                               \
   {                                                                                                               \
     auto kern = rmsnorm_bwd_stream_kernel<XT, WT, CH>;                                                            \
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)             \
-      return B200ATTN_ERR_CUDA;                                                                                   \
+    if (!StreamSmem::allow(kern, 4096)) return B200ATTN_ERR_CUDA;                                                  \
     if (launch_after(kern, dim3(grid), dim3(kBwdStreamThreads), smem, stream, dy, x, w, a->rstd, dx, partial,     \
                      a->rows, a->dim, a->dy_stride_row, a->x_stride_row, a->dx_stride_row, slot,                  \
                      n_slots) != cudaSuccess)                                                                     \
