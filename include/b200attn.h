@@ -496,10 +496,10 @@ int b200attn_kv_append_8bit(const b200attn_kv_append_8bit_args* args, b200attn_s
  * -1 (or any number outside [0, num_pages)) where there is none; page_refs int32
  * [num_pages]: how many rows hold a page, <= 0 for a free one (a caller may add to
  * the count of a page it wants kept).  The results are new tensors, which must not
- * overlap the ones read; entries without a page are -1 there.  Pages are handed out
- * lowest number first, so results are a pure function of the inputs.  A workspace is
- * needed where *_workspace_bytes is not 0.  The reference has no counterpart: its
- * caches are padded and never shared.
+ * overlap the ones read, one another or the workspace (B200ATTN_ERR_SHAPE); entries
+ * without a page are -1 there.  Pages are handed out lowest number first, so results
+ * are a pure function of the inputs.  A workspace is needed where *_workspace_bytes is
+ * not 0.  The reference has no counterpart: its caches are padded and never shared.
  * ---------------------------------------------------------------------- */
 typedef struct {               /* one tensor [num_pages, ...] whose pages are blocks of memory */
   void* base;

@@ -21,6 +21,7 @@
 #include <limits.h>
 
 #include <algorithm>
+#include <initializer_list>
 
 #include "common.cuh"
 #include "sm100.cuh"
@@ -754,21 +755,28 @@ __global__ void __launch_bounds__(kCopyThreads, 2) compact_copy_kernel(const __g
 }
 
 // ---------------------------------------------------------------------------- host side
-bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
-  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
-  return x < y + b_bytes && y < x + a_bytes;
-}
-
 int check_book(const int32_t* table, const int32_t* refs, const int32_t* table_out, const int32_t* refs_out, int slots,
                int width, int pages) {
   if (!table || !refs || !table_out || !refs_out) return B200ATTN_ERR_NULL;
   if (slots <= 0 || width <= 0 || pages <= 0) return B200ATTN_ERR_SHAPE;
   if ((long long)slots * width > INT_MAX) return B200ATTN_ERR_TOO_LARGE;
   if (((uintptr_t)table | (uintptr_t)refs | (uintptr_t)table_out | (uintptr_t)refs_out) & 3) return B200ATTN_ERR_ALIGN;
-  const size_t t = (size_t)slots * width * 4, r = (size_t)pages * 4;
-  if (overlap(table, t, table_out, t) || overlap(refs, r, refs_out, r) || overlap(table, t, refs_out, r) ||
-      overlap(refs, r, table_out, t) || overlap(table_out, t, refs_out, r))
-    return B200ATTN_ERR_SHAPE;
+  return B200ATTN_OK;
+}
+
+// A list of a call's.  The kernels read their inputs again after they have written results, so what is written lies
+// apart from everything else.
+struct Span {
+  const void* at;
+  size_t bytes;
+  bool written;
+};
+int check_apart(std::initializer_list<Span> spans) {
+  for (const Span* a = spans.begin(); a != spans.end(); ++a)
+    for (const Span* b = spans.begin(); b != a; ++b) {
+      const uintptr_t x = (uintptr_t)a->at, y = (uintptr_t)b->at;
+      if ((a->written || b->written) && a->bytes && b->bytes && x < y + b->bytes && y < x + a->bytes) return B200ATTN_ERR_SHAPE;
+    }
   return B200ATTN_OK;
 }
 
@@ -885,7 +893,13 @@ int pages_grow(const b200attn_pages_grow_args* a, cudaStream_t stream) {
                       a->num_pages);
   if (st != B200ATTN_OK) return st;
   if (a->page_size <= 0) return B200ATTN_ERR_SHAPE;
-  st = check_workspace(a->workspace, a->workspace_bytes, pages_grow_workspace_bytes(a));
+  const size_t scratch = pages_grow_workspace_bytes(a), n = (size_t)a->slots * 4;
+  const size_t table = n * a->max_pages_per_seq, counts = (size_t)a->num_pages * 4;
+  st = check_workspace(a->workspace, a->workspace_bytes, scratch);
+  if (st != B200ATTN_OK) return st;
+  st = check_apart({{a->page_table, table, false}, {a->seqlens, n, false}, {a->page_refs, counts, false},
+                    {a->new_tokens, n, false}, {a->page_table_out, table, true}, {a->page_refs_out, counts, true},
+                    {a->missing_out, 4, true}, {a->workspace, scratch, true}});
   if (st != B200ATTN_OK) return st;
   if ((st = device_info(nullptr)) != B200ATTN_OK) return st;
   GrowParams p;
@@ -925,11 +939,15 @@ int pages_fork(const b200attn_pages_fork_args* a, cudaStream_t stream) {
   if (st != B200ATTN_OK) return st;
   if (a->page_size <= 0) return B200ATTN_ERR_SHAPE;
   if (a->slots > kMaxSlots || (long long)a->max_pages_per_seq * a->page_size > INT_MAX) return B200ATTN_ERR_TOO_LARGE;
-  const size_t n = (size_t)a->slots * 4;
-  if (overlap(a->seqlens, n, a->seqlens_out, n) || overlap(a->parents, n, a->seqlens_out, n)) return B200ATTN_ERR_SHAPE;
   st = check_pools(a->pools, a->n_pools);
   if (st != B200ATTN_OK) return st;
-  st = check_workspace(a->workspace, a->workspace_bytes, pages_fork_workspace_bytes(a));
+  const size_t scratch = pages_fork_workspace_bytes(a), n = (size_t)a->slots * 4;
+  const size_t table = n * a->max_pages_per_seq, counts = (size_t)a->num_pages * 4;
+  st = check_workspace(a->workspace, a->workspace_bytes, scratch);
+  if (st != B200ATTN_OK) return st;
+  st = check_apart({{a->page_table, table, false}, {a->seqlens, n, false}, {a->page_refs, counts, false},
+                    {a->parents, n, false}, {a->page_table_out, table, true}, {a->seqlens_out, n, true},
+                    {a->page_refs_out, counts, true}, {a->missing_out, 4, true}, {a->workspace, scratch, true}});
   if (st != B200ATTN_OK) return st;
   const DeviceInfo* di = nullptr;
   if ((st = device_info(&di)) != B200ATTN_OK) return st;
@@ -972,7 +990,12 @@ int pages_compact(const b200attn_pages_compact_args* a, cudaStream_t stream) {
   if (st != B200ATTN_OK) return st;
   st = check_pools(a->pools, a->n_pools);
   if (st != B200ATTN_OK) return st;
-  st = check_workspace(a->workspace, a->workspace_bytes, pages_compact_workspace_bytes(a));
+  const size_t scratch = pages_compact_workspace_bytes(a), counts = (size_t)a->num_pages * 4;
+  const size_t table = (size_t)a->slots * a->max_pages_per_seq * 4;
+  st = check_workspace(a->workspace, a->workspace_bytes, scratch);
+  if (st != B200ATTN_OK) return st;
+  st = check_apart({{a->page_table, table, false}, {a->page_refs, counts, false}, {a->page_table_out, table, true},
+                    {a->page_refs_out, counts, true}, {a->live_out, 4, true}, {a->workspace, scratch, true}});
   if (st != B200ATTN_OK) return st;
   const DeviceInfo* di = nullptr;
   if ((st = device_info(&di)) != B200ATTN_OK) return st;
