@@ -418,7 +418,7 @@ int kv_append_8bit(const b200attn_kv_append_8bit_args* a, cudaStream_t stream) {
   const void* ptrs[4] = {a->new_k, a->new_v, a->k_pages, a->v_pages};
   for (const void* q : ptrs)
     if ((uintptr_t)q & 15) return B200ATTN_ERR_ALIGN;
-  if (((uintptr_t)a->k_scales | (uintptr_t)a->v_scales) & 3) return B200ATTN_ERR_ALIGN;
+  if (!aligned4({a->k_scales, a->v_scales, a->page_table, a->seqlens, a->cu_new})) return B200ATTN_ERR_ALIGN;
   const long long rows[4] = {a->nk_stride_t, a->nk_stride_h, a->nv_stride_t, a->nv_stride_h};
   for (long long s : rows)
     if (s % 8 != 0) return B200ATTN_ERR_STRIDE;

@@ -6,6 +6,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <initializer_list>
+
 #include "../../include/b200attn.h"
 
 namespace b200attn {
@@ -53,6 +55,13 @@ int pages_compact(const b200attn_pages_compact_args* a, cudaStream_t stream);
 int rmsnorm_fwd(const b200attn_rmsnorm_fwd_args* a, cudaStream_t stream);
 size_t rmsnorm_bwd_workspace_bytes(const b200attn_rmsnorm_bwd_args* a);
 int rmsnorm_bwd(const b200attn_rmsnorm_bwd_args* a, cudaStream_t stream);
+
+// whether each of a call's lists of 32-bit numbers starts on one (a list that is not given does)
+inline bool aligned4(std::initializer_list<const void*> lists) {
+  uintptr_t all = 0;
+  for (const void* list : lists) all |= (uintptr_t)list;
+  return (all & 3) == 0;
+}
 
 // Launch allowed to begin while the kernel before it on the stream drains; the kernel itself waits
 // (sm100::grid_dependency_wait) before it touches global memory.  Its set-up and the launch gap then

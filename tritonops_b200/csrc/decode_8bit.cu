@@ -768,7 +768,8 @@ int validate(const b200attn_paged_decode_8bit_args* a) {
   const void* ptrs[3] = {a->q, a->k_pages, a->v_pages};
   for (const void* ptr : ptrs)
     if ((uintptr_t)ptr & 15) return B200ATTN_ERR_ALIGN;
-  if (((uintptr_t)a->o & 1) || (((uintptr_t)a->k_scales | (uintptr_t)a->v_scales) & 3)) return B200ATTN_ERR_ALIGN;
+  if (((uintptr_t)a->o & 1) || !aligned4({a->k_scales, a->v_scales, a->page_table, a->seqlens, a->status_word}))
+    return B200ATTN_ERR_ALIGN;
   const long long rows[3] = {a->q_stride_b, a->q_stride_t, a->q_stride_h};
   for (long long s : rows)
     if (s % 8 != 0) return B200ATTN_ERR_STRIDE;

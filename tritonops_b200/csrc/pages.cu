@@ -760,8 +760,7 @@ int check_book(const int32_t* table, const int32_t* refs, const int32_t* table_o
   if (!table || !refs || !table_out || !refs_out) return B200ATTN_ERR_NULL;
   if (slots <= 0 || width <= 0 || pages <= 0) return B200ATTN_ERR_SHAPE;
   if ((long long)slots * width > INT_MAX) return B200ATTN_ERR_TOO_LARGE;
-  if (((uintptr_t)table | (uintptr_t)refs | (uintptr_t)table_out | (uintptr_t)refs_out) & 3) return B200ATTN_ERR_ALIGN;
-  return B200ATTN_OK;
+  return aligned4({table, refs, table_out, refs_out}) ? B200ATTN_OK : B200ATTN_ERR_ALIGN;
 }
 
 // A list of a call's.  The kernels read their inputs again after they have written results, so what is written lies
@@ -893,6 +892,7 @@ int pages_grow(const b200attn_pages_grow_args* a, cudaStream_t stream) {
                       a->num_pages);
   if (st != B200ATTN_OK) return st;
   if (a->page_size <= 0) return B200ATTN_ERR_SHAPE;
+  if (!aligned4({a->seqlens, a->new_tokens, a->missing_out})) return B200ATTN_ERR_ALIGN;
   const size_t scratch = pages_grow_workspace_bytes(a), n = (size_t)a->slots * 4;
   const size_t table = n * a->max_pages_per_seq, counts = (size_t)a->num_pages * 4;
   st = check_workspace(a->workspace, a->workspace_bytes, scratch);
@@ -939,6 +939,7 @@ int pages_fork(const b200attn_pages_fork_args* a, cudaStream_t stream) {
   if (st != B200ATTN_OK) return st;
   if (a->page_size <= 0) return B200ATTN_ERR_SHAPE;
   if (a->slots > kMaxSlots || (long long)a->max_pages_per_seq * a->page_size > INT_MAX) return B200ATTN_ERR_TOO_LARGE;
+  if (!aligned4({a->seqlens, a->parents, a->seqlens_out, a->missing_out})) return B200ATTN_ERR_ALIGN;
   st = check_pools(a->pools, a->n_pools);
   if (st != B200ATTN_OK) return st;
   const size_t scratch = pages_fork_workspace_bytes(a), n = (size_t)a->slots * 4;
@@ -988,6 +989,7 @@ int pages_compact(const b200attn_pages_compact_args* a, cudaStream_t stream) {
   int st = check_book(a->page_table, a->page_refs, a->page_table_out, a->page_refs_out, a->slots, a->max_pages_per_seq,
                       a->num_pages);
   if (st != B200ATTN_OK) return st;
+  if (!aligned4({a->live_out})) return B200ATTN_ERR_ALIGN;
   st = check_pools(a->pools, a->n_pools);
   if (st != B200ATTN_OK) return st;
   const size_t scratch = pages_compact_workspace_bytes(a), counts = (size_t)a->num_pages * 4;
