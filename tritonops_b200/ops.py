@@ -108,9 +108,10 @@ def _need_cuda(*ts):
 def _rowmajor16(t: Tensor) -> Tensor:
     """Keep arbitrary outer strides (the reference passes all strides through,
     flash_attn_triton.py:633-646) but require unit inner stride and 16-byte
-    addressable rows; copy otherwise."""
+    addressable rows; copy otherwise, what torch calls contiguous (from an odd base, or with an axis
+    of one and any stride there) as well."""
     ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in t.stride()[:-1])
-    return t if ok else t.contiguous()
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
 
 
 def _ptr(t: Optional[Tensor]):
