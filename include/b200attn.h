@@ -42,11 +42,11 @@ typedef struct CUstream_st* b200attn_stream_t; /* == cudaStream_t */
 typedef enum {
   B200ATTN_OK = 0,
   B200ATTN_ERR_NULL = -1,        /* a required pointer is NULL */
-  B200ATTN_ERR_DTYPE = -2,       /* dtype is not F16 / BF16 */
+  B200ATTN_ERR_DTYPE = -2,       /* dtype is not F16 / BF16 (a cache in 8 bits: E4M3 / I8) */
   B200ATTN_ERR_HEAD_DIM = -3,    /* head_dim not in {32, 64, 96, 128} */
   B200ATTN_ERR_GQA = -4,         /* heads_q not a positive multiple of heads_kv */
-  B200ATTN_ERR_ALIGN = -5,       /* base pointer not 16-byte aligned */
-  B200ATTN_ERR_STRIDE = -6,      /* a stride is not a multiple of 8 elements (16 bytes) */
+  B200ATTN_ERR_ALIGN = -5,       /* base pointer not 16-byte aligned, or a list of 32-bit numbers not 4-byte */
+  B200ATTN_ERR_STRIDE = -6,      /* a stride is not a multiple of 16 bytes, or 0 where numbers must lie apart */
   B200ATTN_ERR_SHAPE = -7,       /* negative / zero / inconsistent sizes */
   B200ATTN_ERR_WORKSPACE = -8,   /* workspace missing or too small */
   B200ATTN_ERR_MODE = -9,        /* unknown sparsity mode or bad window / block parameters */
@@ -452,8 +452,11 @@ size_t b200attn_paged_decode_8bit_workspace_bytes(const b200attn_paged_decode_8b
  * of `queries` attends to keys t < len - queries + 1 + i (the token itself and
  * what came before it), len cut at max_seqlen and at the row of the page table.
  * A query without a visible key gives 0.  Scores, softmax statistics and sums
- * are fp32; Q enters the products as fp16 (bf16 rows scaled by a power of two
- * first), the cached numbers as fp16, which holds them exactly. */
+ * are fp32.  The products take fp16 operands: the cached numbers, exact; Q (bf16
+ * rows scaled by a power of two first, so that an element below 2^-14 of its row's
+ * largest is rounded to 2^-25 of that); and the softmax weights, rounded to fp16's
+ * 11 bits, 2^-11 relative, down to 2^-24 of the row's largest weight.  The sum they
+ * are divided by is of the unrounded weights. */
 int b200attn_paged_decode_8bit_fwd(const b200attn_paged_decode_8bit_args* args, b200attn_stream_t stream);
 
 typedef struct {
@@ -551,7 +554,8 @@ size_t b200attn_pages_fork_workspace_bytes(const b200attn_pages_fork_args* args)
  * that takes it); the others share its full pages and get a copy, in every pool, of the
  * last page if that is only partly filled.  Pages that no row holds any more are free,
  * also for the copies of this call.  A copy that finds no free page is left out: its
- * entry is -1, its length is cut to the full pages and missing_out counts it. */
+ * entry is -1, its length is cut to the full pages and missing_out counts it.  At most
+ * 32768 slots, and rows of at most 2^31 - 1 tokens (B200ATTN_ERR_TOO_LARGE). */
 int b200attn_pages_fork(const b200attn_pages_fork_args* args, b200attn_stream_t stream);
 
 typedef struct {
@@ -570,7 +574,8 @@ typedef struct {
 size_t b200attn_pages_compact_workspace_bytes(const b200attn_pages_compact_args* args);
 
 /* The pages in use moved to the front of every pool: with n of them, those at n and
- * beyond take, in order, the free places below n. */
+ * beyond take, in order, the free places below n.  A page that only its count keeps is
+ * moved like the others; where it went can be read from a row of the table that lists it. */
 int b200attn_pages_compact(const b200attn_pages_compact_args* args, b200attn_stream_t stream);
 
 /* ------------------------------------------------------------------------

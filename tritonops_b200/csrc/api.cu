@@ -55,11 +55,11 @@ const char* b200attn_strerror(int status) {
   switch (status) {
     case B200ATTN_OK: return "ok";
     case B200ATTN_ERR_NULL: return "a required pointer is NULL (or both / neither of cu_seqlens and seqlens given)";
-    case B200ATTN_ERR_DTYPE: return "dtype must be fp16 or bf16";
+    case B200ATTN_ERR_DTYPE: return "dtype must be fp16 or bf16 (a cache in 8 bits: e4m3 or int8)";
     case B200ATTN_ERR_HEAD_DIM: return "head_dim must be 32, 64, 96 or 128";
     case B200ATTN_ERR_GQA: return "heads_q must be a positive multiple of heads_kv";
-    case B200ATTN_ERR_ALIGN: return "base pointer is not 16-byte aligned";
-    case B200ATTN_ERR_STRIDE: return "stride is not a multiple of 8 elements";
+    case B200ATTN_ERR_ALIGN: return "a pointer is not aligned (tensors to 16 bytes, lists and scales to 4)";
+    case B200ATTN_ERR_STRIDE: return "a stride is not a multiple of 16 bytes, or is 0 where numbers must lie apart";
     case B200ATTN_ERR_SHAPE: return "invalid or inconsistent sizes";
     case B200ATTN_ERR_WORKSPACE: return "workspace missing or too small";
     case B200ATTN_ERR_MODE: return "bad sparsity mode, window or block-list parameters";

@@ -25,8 +25,14 @@
 // 0.85.  Up to 8 query rows the memory bounds it.  With 16 the warps' own chain does (43 % of the issue slots,
 // two warps a scheduler, 168 registers): 32 sequences of 4096 keys take 87 us against 42 us for their bytes,
 // and more rows take another pass (20 rows: 140 us).  24 rows at once with Q in shared memory spilled: 174 us.
-// bf16 queries are scaled by a power of two per row so that fp16 holds them; P is 2^10 times the
-// weight, which keeps weights down to 2^-24 of the largest one out of fp16's subnormals.
+// The products take 16-bit operands, and of the types fp16 holds the cached numbers exactly, so the other
+// operand is rounded to its 11 bits too (the rest of either would be a second product for each):
+//   * Q: fp16 rows as they are; bf16 rows (8 bits) times a power of two per row, exact but for what lies below
+//     2^-14 of the row's largest element, which is rounded to 2^-25 of that.
+//   * P, 2^10 times the weight, which keeps weights down to 2^-24 of the largest one out of fp16's
+//     subnormals: relative 2^-11 of a weight; the sum of weights is of the unrounded ones, in fp32.  The
+//     outputs' relative error against 64 bits is 2.1e-4 (fp16, 333 keys) and 2.2e-4 (20 rows of drafts), where
+//     32-bit arithmetic has 2.0e-4 and 2.1e-4; 1.7e-3 either way for bf16 outputs, whose own rounding that is.
 #include <limits.h>
 
 #include <algorithm>
@@ -800,6 +806,7 @@ int chunk_of(const b200attn_paged_decode_8bit_args* a) {
   if (a->chunk_tokens > 0) return a->chunk_tokens;
   const long long units = a->batch * (long long)a->heads_kv * ((rows_of(a) + kRowsTile - 1) / kRowsTile);
   const long long stages = std::max<long long>((max_visible(a) + kStageKeys - 1) / kStageKeys, 1);
+  // (148: the chip's SMs.  The workspace follows from the split and can be asked for without a device.)
   const long long slots = 148 * ctas_per_sm(a->head_dim, (int)std::min<long long>(rows_of(a), kRowsTile));
   long long best = 0, least = 0;
   auto consider = [&](long long per) {

@@ -6,9 +6,12 @@
 // move where is an ordered enumeration (the i-th free page for the i-th place that needs one), so
 // the results are a pure function of the inputs.  The host fetches nothing, and the steps of one call
 // depend on one another, so there are two forms:
-//   * Where a CTA can keep the bookkeeping in shared memory (up to some ten thousand pages), every CTA of
-//     the copying grid works it out for itself from the same inputs, writes its share of the new tables
-//     and copies its share of the pages: one launch, nothing exchanged.
+//   * Where a CTA can keep the bookkeeping in shared memory (a fork: pages + 8 slots up to 28,672; a
+//     compaction: 14,335 pages; a hand-out: pages + 3 slots up to 12,288, and 16,384 of pages and table
+//     entries together, where one CTA does it all), every CTA of the copying grid works it out for itself
+//     from the same inputs, writes its share of the new tables and copies its share of the pages: one
+//     launch, nothing exchanged.  Each CTA of a fork reads the whole table for that, which rows much wider
+//     than what they hold make dear.
 //   * Beyond, a fork's or compaction's books are kept by one cluster of CTAs (cluster barriers between the
 //     steps: a few hundred nanoseconds, against microseconds for a launch) and a second kernel copies from
 //     its list; a hand-out, which copies nothing, spreads the tables over the chip in two launches.
@@ -16,8 +19,11 @@
 //   hand-out    8 rows of 63 entries 4.1 us (one CTA); 1024 rows of 537 entries and 327,000 pages 11.0 us,
 //               33.9 us by one cluster: 2 MB of table through eight SMs
 //   fork        one sequence into four 7.3 us; 64 into 256, 40 MB copied, 22.4 us: 8 us of launch and books (a
-//               chain of look-ups and barriers) and the copies, whose floor is 12.3 us
-//   compaction  47 small pages 4.7 us; 0.79 GB moved 275 us, 5.8 TB/s = 0.89 of a copy (both tables included)
+//               chain of look-ups and barriers) and the copies, whose floor is 12.3 us.  256 slots that hold 24 pages
+//               each, books alone: rows of 24 entries 12.1 us, 512 68.6, 2048 247, 8192 957.  By a cluster: 1024 slots,
+//               rows of 537, 332,538 pages 67.5 us
+//   compaction  47 small pages 4.7 us; 0.79 GB moved 275 us, 5.8 TB/s = 0.89 of a copy (both tables included).  By a
+//               cluster, the books just named, alone: 93 us
 #include <limits.h>
 
 #include <algorithm>
@@ -32,7 +38,7 @@ namespace {
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanCtas = 8;             // the largest portable cluster
 constexpr int kMaxSlots = 32768;         // slots of a fork: their keepers stay in shared memory
-constexpr int kHeader = 64;              // ints at the front of every workspace
+constexpr int kHeader = 64;              // ints at the front of a fork's or compaction's workspace
 constexpr int kCopies = 0, kCountA = 8, kCountB = 24, kCountC = 40;   // in the header: copies, counts per CTA
 
 __device__ __forceinline__ int cluster_rank() {
@@ -250,6 +256,7 @@ struct GrowGridParams {
   GrowShare* shares;         // [kGrowCtas]
   int rows_each, pages_each; // shares
 };
+// (Two for each SM of the chip; any number is right.  A constant, as the workspace is asked for without a device.)
 constexpr int kGrowCtas = 2 * 148, kGrowThreads = 256;
 
 __global__ void __launch_bounds__(kGrowThreads) grow_look_kernel(const GrowGridParams q) {
